@@ -1,0 +1,5 @@
+// Gated feed-forward products of bf16 operands.
+#include "ffn_gated_launch.hpp"
+namespace zluda_amd {
+uint32_t launch_gated_bf16(const GatedParams &p, hipStream_t s) { return launch_gated<ElemBF16>(p, s); }
+} // namespace zluda_amd

@@ -1,0 +1,115 @@
+// Element by element: storing and loading checkpoints, and the gradients of the gated activation (include/zluda_ffn.h).
+// All memory bound.  A thread owns eight neighbouring columns (16 bytes of a 16-bit type, eight codes) and walks rows; 64
+// threads side by side, four rows at a time in a workgroup.
+#pragma once
+#include "ffn_common.hpp"
+
+namespace zluda_amd {
+
+struct CheckpointParams {
+  void *x;
+  uint8_t *codes, *scales;
+  int64_t rows, ldx, ld_codes, ld_scales;
+  int32_t cols;
+};
+
+template <class E>
+__global__ __launch_bounds__(256) void checkpoint_store_kernel(CheckpointParams p) {
+  const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63)), cols32 = (p.cols + 31) & ~31;
+  for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < p.rows; row += gridDim.y * 4) {  // (whole waves)
+    const typename E::Raw8 r = load8<E>((const typename E::raw *)p.x + row * p.ldx + col, p.cols - col);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = E::get(r, e);
+    ckpt_store8(p.codes + row * p.ld_codes, p.scales + row * p.ld_scales, col, cols32, v);
+  }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void checkpoint_load_kernel(CheckpointParams p) {
+  const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63));
+  if (col >= p.cols) return;
+  for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < p.rows; row += gridDim.y * 4) {
+    float v[8];
+    ckpt_get8(ckpt_load8(p.codes + row * p.ld_codes, p.scales + row * p.ld_scales, col), v);
+    store8<E>((typename E::raw *)p.x + row * p.ldx + col, v, p.cols - col);
+  }
+}
+
+struct GatedGradParams {
+  const void *dh, *gate, *up;              // gate, up: elements or codes
+  const uint8_t *gate_scales, *up_scales;  // of checkpoints
+  void *dz, *h;                            // dz: [dG dU]; h or NULL
+  float *part;                             // [gridDim.y][2 * features]: partial sums of dz over the rows, or NULL
+  int64_t tokens, lddh, ldg, ldu, ldgs, ldus, lddz, ldh;
+  int32_t features;
+  uint32_t activation;
+};
+
+// dU = dH act(G), dG = dH U act'(G); H = act(G) U on request.  CK: gate and up are checkpoints.
+template <class E, bool CK, int ACT>
+__global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
+  using raw = typename E::raw;
+  const int lane = threadIdx.x & 63, phase = threadIdx.x >> 6, col = 8 * (blockIdx.x * 64 + lane), n = p.features - col;
+  float sg[8], su[8];
+#pragma unroll
+  for (int e = 0; e < 8; e++) sg[e] = su[e] = 0.0f;
+  if (n > 0) {
+    for (int64_t row = blockIdx.y * 4 + phase; row < p.tokens; row += gridDim.y * 4) {
+      float g[8], u[8], dg[8], du[8];
+      const typename E::Raw8 rd = load8<E>((const raw *)p.dh + row * p.lddh + col, n);
+      if constexpr (CK) {
+        ckpt_get8(ckpt_load8((const uint8_t *)p.gate + row * p.ldg, p.gate_scales + row * p.ldgs, col), g);
+        ckpt_get8(ckpt_load8((const uint8_t *)p.up + row * p.ldu, p.up_scales + row * p.ldus, col), u);
+      } else {
+        const typename E::Raw8 rg = load8<E>((const raw *)p.gate + row * p.ldg + col, n), ru = load8<E>((const raw *)p.up + row * p.ldu + col, n);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          g[e] = E::get(rg, e);
+          u[e] = E::get(ru, e);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        float a, da;
+        ffn_act_grad<ACT>(g[e], a, da);
+        const float d = E::get(rd, e);
+        dg[e] = d * u[e] * da;
+        du[e] = d * a;
+        g[e] = a * u[e];
+        sg[e] += dg[e];
+        su[e] += du[e];
+      }
+      store8<E>((raw *)p.dz + row * p.lddz + col, dg, n);
+      store8<E>((raw *)p.dz + row * p.lddz + p.features + col, du, n);
+      if (p.h) store8<E>((raw *)p.h + row * p.ldh + col, g, n);
+    }
+  }
+  if (!p.part) return;
+  __shared__ float fold[4][2][8][64];
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    fold[phase][0][e][lane] = sg[e];
+    fold[phase][1][e][lane] = su[e];
+  }
+  __syncthreads();
+  for (int o = threadIdx.x; o < 2 * 8 * 64; o += 256) {
+    const int which = o >> 9, e = (o >> 6) & 7, l = o & 63, c = 8 * (blockIdx.x * 64 + l) + e;
+    if (c < p.features)
+      p.part[(int64_t)blockIdx.y * 2 * p.features + which * p.features + c] =
+          (fold[0][which][e][l] + fold[1][which][e][l]) + (fold[2][which][e][l] + fold[3][which][e][l]);
+  }
+}
+
+// zeros where a sum has no terms (no memset node: those have replayed wrongly in captured graphs)
+struct ZeroParams {
+  void *p;
+  int64_t rows, row_bytes, pitch_bytes;  // multiples of 2
+};
+__global__ __launch_bounds__(256) void zero_rows_kernel(ZeroParams z) {
+  const int64_t words = z.row_bytes / 2;
+  for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < z.rows * words; i += (int64_t)gridDim.x * 256)
+    ((uint16_t *)((char *)z.p + i / words * z.pitch_bytes))[i % words] = 0;
+}
+
+} // namespace zluda_amd
