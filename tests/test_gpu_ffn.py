@@ -138,6 +138,17 @@ def test_gated_forward_sizes(gpu_api, typ, t, d, f):
             check_gated(h, g, u, kept, ref, what)
 
 
+# enough tiles for the persistent kernel: ragged in every direction, K of two stages, of an odd number, with a tail
+@pytest.mark.parametrize("t,d,f", [(1100, 200, 3400), (1025, 72, 3401), (2049, 64, 2056), (769, 328, 4100), (300, 512, 8200)])
+@pytest.mark.parametrize("typ,act,kept", [("bf16", "silu", ffn.KEPT_8BIT), ("f16", "gelu", ffn.KEPT_PLAIN), ("bf16", "relu", ffn.KEPT_NONE)])
+def test_gated_forward_many_tiles(gpu_api, t, d, f, typ, act, kept):
+    for bias, skip in ((True, 0), (False, 0), (True, 8)):
+        what = "gated %s %s %d x %d x %d kept %d" % (typ, act, t, d, f, kept)
+        print(what, flush=True)
+        _, _, _, h, g, u, ref = run_gated(typ, act, t, d, f, bias, kept, skip, skip, seed=t)
+        check_gated(h, g, u, kept, ref, what)
+
+
 @pytest.mark.parametrize("pad,skip", [(0, 1), (1, 0), (3, 5), (8, 0), (8, 8), (4, 4)])
 @pytest.mark.parametrize("t,d,f", [(1, 128, 64), (9, 80, 72), (150, 256, 160), (520, 192, 264)])
 def test_gated_forward_pitches_and_alignments(gpu_api, t, d, f, pad, skip):

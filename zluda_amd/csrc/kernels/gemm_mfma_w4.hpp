@@ -48,7 +48,11 @@ __device__ __forceinline__ bool w4_stream_d_i32(const GemmArgs &g) {
 }
 
 // the epilogue an instantiation carries; the planner sends it the problems that one serves (w4_epilogue_class)
-enum { W4_EPI_I32 = 0, W4_EPI_BF16 = 1, W4_EPI_BF16_GELU = 2, W4_EPI_GELU_AUX = 3 };  // (the last: GELU with its input kept, 16-bit D)
+enum { W4_EPI_I32 = 0, W4_EPI_BF16 = 1, W4_EPI_BF16_GELU = 2, W4_EPI_GELU_AUX = 3,  // (the last: GELU with its input kept, 16-bit D)
+       // A gated layer (16-bit operands; Params: GatedMfmaParams of ffn_gated_w4.hpp): A holds 2 M rows, and the tile's P rows are
+       // 128 of the first M and the 128 of the second M that belong to them, 64 and 64 in each wave's share, so that a lane
+       // holds both products of an output element.
+       W4_EPI_GATED = 4 };
 
 // one accumulator element, AGPR -> VGPR
 template <class T>
@@ -393,8 +397,9 @@ __device__ __forceinline__ void w4_store_i32(const MfmaParams &prm, AccV (&acc)[
   }
 }
 
-template <int KIND, int FQ, int FP, int EPI>
-__global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(MfmaParams prm) {
+template <int KIND, int FQ, int FP, int EPI, class Params = MfmaParams>
+__global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
+  constexpr bool GATED = EPI == W4_EPI_GATED;
   static_assert(KIND == KIND_I8 || KIND == KIND_F8 || KIND == KIND_MXF4 || kind_is_h16(KIND), "int8, fp8, MXFP4, f16 and bf16 operands");
   constexpr bool H16 = kind_is_h16(KIND);  // v_mfma_f32_16x16x32_f16 / _bf16: the byte geometry of int8 (16 bytes of K per lane and K step)
   constexpr bool MX = KIND == KIND_MXF4;
@@ -446,7 +451,7 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(MfmaParams prm) {
   // n-th tile of this workgroup -> tile corner and batch (G is a multiple of 8 whenever a workgroup has more than one tile)
   auto tile_coords = [&](int n, int &p0, int &q0, int &bt) __attribute__((always_inline)) {
     const WorkItem it = work_item(prm, blockIdx.x + (uint32_t)(n * G));
-    p0 = it.p * BP;
+    p0 = it.p * (GATED ? BP / 2 : BP);
     q0 = it.q * BQ;
     bt = it.bt;
   };
@@ -510,7 +515,12 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(MfmaParams prm) {
     rsP = __builtin_amdgcn_make_buffer_rsrc((void *)Pg, 0, 0x80000000, 0x00020000);
     rsQ = __builtin_amdgcn_make_buffer_rsrc((void *)Qg, 0, 0x80000000, 0x00020000);
 #pragma unroll
-    for (int i = 0; i < LP; i++) voffP[i] = min(p0 + drow + RPP * i, NP - 1) * ldp + dcg * 16;
+    for (int i = 0; i < LP; i++) {
+      if constexpr (GATED)  // (i / 4: the wave share, i % 4: its rows in steps of 32, two of each half of A)
+        voffP[i] = (min(p0 + (WTP / 2) * (i / 4) + drow + RPP * (i & 1), NP - 1) + ((i & 2) ? NP : 0)) * ldp + dcg * 16;
+      else
+        voffP[i] = min(p0 + drow + RPP * i, NP - 1) * ldp + dcg * 16;
+    }
 #pragma unroll
     for (int i = 0; i < LQ; i++) voffQ[i] = min(q0 + drow + RPP * i, NQ - 1) * ldq + dcg * 16;
     scale_tile(n, p0, q0, bt);
@@ -790,6 +800,8 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(MfmaParams prm) {
     if constexpr (EPI == W4_EPI_I32) {
       if (stream_d) w4_store_i32<WTP, WTQ, 2>(prm, acc, p0, q0, NP, NQ, bt, wp, wq, ialpha);
       else w4_store_i32<WTP, WTQ, 0>(prm, acc, p0, q0, NP, NQ, bt, wp, wq, ialpha);
+    } else if constexpr (GATED) {
+      prm.store_tile(acc, p0 + wp * (WTP / 2), q0 + wq * WTQ, staged);
     } else {
       constexpr int ACT = EPI == W4_EPI_BF16_GELU || EPI == W4_EPI_GELU_AUX ? ACT_GELU : ACT_NONE;
       constexpr bool KEPT = EPI == W4_EPI_GELU_AUX;
@@ -812,7 +824,20 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(MfmaParams prm) {
   // staging area: requested at the top of the tile, landed by the vmcnt(0) waits of the tile's last two stages (there
   // always are two).  Only the wave itself reads them, after those waits and before it requests the next tile's.
   auto stage_vectors = [&](int p0, int q0, int bt) __attribute__((always_inline)) {
-    if constexpr (EPI != W4_EPI_I32 && !MX) {
+    if constexpr (GATED) {
+      // the biases of the wave's 64 features: Wg's in slot 0, Wu's in slot 1, each from the dword that holds its first element
+      const int pc = p0 + wp * (WTP / 2), pn = min(WTP / 2, NP - pc);
+      if (g.bias != nullptr && pn > 0) {
+        int *const area = (int *)&lds[2 * STAGE_V4] + wave * STG_WAVE;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const char *src = (const char *)g.bias + ((int64_t)h * NP + pc) * 2;
+          const int skip = (int)(((uintptr_t)src) & 3);
+          const __amdgpu_buffer_rsrc_t rsv = __builtin_amdgcn_make_buffer_rsrc((void *)(src - skip), 0, (pn * 2 + skip + 3) & ~3, 0x00020000);
+          lds_dma4(rsv, area + h * W4Staged::WORDS, lane_here() * 4, 0);
+        }
+      }
+    } else if constexpr (EPI != W4_EPI_I32 && !MX) {
       staged.has[0] = staged.has[1] = staged.has[2] = staged.has[3] = staged.has[4] = false;
       staged.bias_skip = 0;
       {
