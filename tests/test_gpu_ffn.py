@@ -138,6 +138,17 @@ def test_gated_forward_sizes(gpu_api, typ, t, d, f):
             check_gated(h, g, u, kept, ref, what)
 
 
+# every tile of gated_tile(): one, two and three token rows of each, K with a tail, of an odd number of stages, shorter than the ring
+@pytest.mark.parametrize("t,d,f", [(7, 328, 4100), (33, 64, 4100), (50, 200, 8200), (65, 8, 4100), (120, 328, 12000), (128, 64, 12000), (257, 328, 6000), (250, 136, 12800)])
+@pytest.mark.parametrize("typ,act,kept", [("bf16", "silu", ffn.KEPT_8BIT), ("f16", "gelu", ffn.KEPT_PLAIN), ("bf16", "relu", ffn.KEPT_NONE)])
+def test_gated_forward_tiles(gpu_api, t, d, f, typ, act, kept):
+    for bias, skip in ((True, 0), (False, 8)):
+        what = "gated %s %s %d x %d x %d kept %d" % (typ, act, t, d, f, kept)
+        print(what, flush=True)
+        _, _, _, h, g, u, ref = run_gated(typ, act, t, d, f, bias, kept, skip, skip, seed=t)
+        check_gated(h, g, u, kept, ref, what)
+
+
 # enough tiles for the persistent kernel: ragged in every direction, K of two stages, of an odd number, with a tail
 @pytest.mark.parametrize("t,d,f", [(1100, 200, 3400), (1025, 72, 3401), (2049, 64, 2056), (769, 328, 4100), (300, 512, 8200)])
 @pytest.mark.parametrize("typ,act,kept", [("bf16", "silu", ffn.KEPT_8BIT), ("f16", "gelu", ffn.KEPT_PLAIN), ("bf16", "relu", ffn.KEPT_NONE)])

@@ -1,4 +1,4 @@
-// Gated feed-forward products of bf16 operands.
+// Gated feed-forward products of bf16 operands on the four-wave persistent kernel, and the choice between it and the others.
 #include "ffn_gated_launch.hpp"
 namespace zluda_amd {
 uint32_t launch_gated_bf16(const GatedParams &p, hipStream_t s) { return launch_gated<ElemBF16>(p, s); }

@@ -4,7 +4,6 @@
 
 #include "../../include/zluda_gemm_launch.h"
 #include "ffn_launch.hpp"
-#include "kernels/ffn_gated_any.hpp"
 #include "kernels/ffn_gated_w4.hpp"
 
 namespace zluda_amd {
@@ -32,13 +31,31 @@ inline uint32_t launch_gated_w4(const GatedParams &p, int cus, hipStream_t s) {
   return launch_kernel(gemm_mfma_w4_kernel<KIND, 0, 0, W4_EPI_GATED, GatedMfmaParams<E>>, dim3((uint32_t)(tiles < slots ? tiles : slots)), dim3(256), s, m);
 }
 
+// The tile whose slowest CU is done first: rounds of tiles over the CUs, each the stages of K (and the time of three for its
+// start and end).  All tiles share the bound of the one read of W, under which their differences vanish.
+// Measured and predicted best, us (64 x 32, 64 x 64, 64 x 128, 128 x 128, 128 x 256 persistent): 300 tokens, 2048 x 5632: 34, 22, 36,
+// 30, 43; 256 tokens, 4096 x 14336: 135, 106, 89, 74, 122; 512 tokens: 235, 172, 163, 131, 122; 64 tokens: 56, 46, 50, 63, 94.
+inline int gated_tile(const GatedParams &p, int cus) {
+  const int stages = (p.model + 63) / 64 + 3;
+  int best = 0;
+  float best_us = 0.0f;
+  for (int v = 0; v < kGatedTileCount; v++) {
+    const GatedTile &t = kGatedTiles[v];
+    const int64_t n = ((p.features + t.features - 1) / t.features) * (int64_t)((p.tokens + t.tokens - 1) / t.tokens);
+    const float us = (float)((n + cus - 1) / cus) * t.stage_us * stages;
+    if (v == 0 || us < best_us) {
+      best = v;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
 template <class E>
 inline uint32_t launch_gated(const GatedParams &p, hipStream_t s) {
-  const int cus = (int)zluda_gemm_device_cu_count();
-  const int64_t tiles = ((p.features + 127) / 128) * (int64_t)((p.tokens + 255) / 256);
-  if (gated_dma_operands(p) && tiles >= cus / 2) return launch_gated_w4<E>(p, cus, s);
-  const dim3 grid((p.features + 31) / 32, (p.tokens + 63) / 64);
-  return launch_kernel(gated_any_kernel<E>, grid, dim3(256), s, p);
+  const int cus = (int)zluda_gemm_device_cu_count(), tile = gated_dma_operands(p) ? gated_tile(p, cus) : -1;
+  if (tile == kGatedPersistent) return launch_gated_w4<E>(p, cus, s);
+  return E::type == CUDA_R_16BF ? launch_gated_small_bf16(p, tile, s) : launch_gated_small_f16(p, tile, s);
 }
 
 } // namespace zluda_amd
