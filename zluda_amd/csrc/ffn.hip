@@ -77,11 +77,13 @@ struct GradPlan {
   uint32_t shares;                    // partial rows of dbias
 };
 
-// workgroups along the rows for kernels whose workgroup takes `strips` pieces of a row side by side and `rows_each` rows at a
-// time: about eight workgroups a CU over all
-uint32_t row_groups(uint64_t rows, int strips, int rows_each, int per_cu) {
-  const uint64_t want = std::max<uint64_t>(1, ((uint64_t)cus() * per_cu + strips - 1) / strips), most = (rows + rows_each - 1) / rows_each;
-  return (uint32_t)std::min<uint64_t>({want, std::max<uint64_t>(most, 1), kGridY});
+// Workgroups of gated_grad_kernel along the rows.  Without sums a row of its own for every thread (8192 x 8192: 112 us, 130 with eight
+// workgroups a CU that walk the rows); with them at least four rows a thread and at most eight workgroups a CU, because each
+// leaves a row of partial sums (1001 x 2816: 10.9 us, 15.4 with one row a thread).
+uint32_t grad_shares(uint64_t tokens, uint64_t features, bool sums) {
+  const uint64_t strips = (features + 511) / 512, each = sums ? 16 : 4, most = std::max<uint64_t>(1, (tokens + each - 1) / each);
+  const uint64_t want = sums ? std::max<uint64_t>(1, ((uint64_t)cus() * 8 + strips - 1) / strips) : most;
+  return (uint32_t)std::min<uint64_t>({want, most, kGridY});
 }
 
 GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
@@ -89,7 +91,7 @@ GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
   memset(&g, 0, sizeof(g));
   uint64_t at = 0;
   g.lddz = p->dz.data ? p->dz.ld : (int64_t)((2 * p->features + 7) & ~7ull);
-  g.shares = row_groups(p->tokens, (int)((p->features + 511) / 512), 4, 8);
+  g.shares = grad_shares(p->tokens, p->features, p->dbias != nullptr);
   g.dz = at;
   if (!p->dz.data) at += aligned256(p->tokens * (uint64_t)g.lddz * 2);
   g.x = at;
@@ -126,8 +128,7 @@ uint32_t check_backward(const zluda_ffn_gated_grad *p) {
 
 template <class E>
 uint32_t launch_checkpoint(bool store, const CheckpointParams &p, hipStream_t s) {
-  const int strips = (p.cols + 511) / 512;
-  const dim3 grid(strips, row_groups((uint64_t)p.rows, strips, 4, 16));
+  const dim3 grid((p.cols + 511) / 512, (uint32_t)std::min<int64_t>((p.rows + 3) / 4, kGridY));
   return store ? launch_kernel(checkpoint_store_kernel<E>, grid, dim3(256), s, p) : launch_kernel(checkpoint_load_kernel<E>, grid, dim3(256), s, p);
 }
 
@@ -210,20 +211,22 @@ uint32_t launch_norm(const NormParams &p, hipStream_t s) {
   return launch_kernel(norm_forward_kernel<E, 1024, 1, 2>, groups(1, 2), dim3(1024), s, p);
 }
 
-// rows a workgroup of the gradient kernel takes at a time, and workgroups
-int norm_grad_rows_each(uint64_t cols) { return cols <= 1024 ? 8 : cols <= 4096 ? 2 : 1; }
+// Rows a workgroup of the gradient kernel takes at a time, and workgroups: two a CU (one of 1024 threads), each with at least two
+// rounds of rows, because every workgroup's partial sums are written and read again (us with at least 1, 2, 4, 8 rounds: 300 x 4096
+// bf16 12.2, 10.6, 11.1, 13.3; 777 x 1001 f16 10.1, 10.0, 11.5, 16.2; 500 x 16384 50.1, 35.2, 29.1, 35.0)
+int norm_grad_rows_each(uint64_t cols) { return cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1; }
 uint32_t norm_grad_groups(uint64_t rows, uint64_t cols) {
-  const int each = norm_grad_rows_each(cols);
-  return (uint32_t)std::min<uint64_t>((rows + each - 1) / each, (uint64_t)cus() * 2);
+  const int least = norm_grad_rows_each(cols) * (cols <= 8192 ? 2 : 4);
+  return (uint32_t)std::min<uint64_t>((rows + least - 1) / least, (uint64_t)cus() * (cols <= 4096 ? 2 : 1));
 }
 
 template <class E, bool CK>
 uint32_t launch_norm_grad(const NormGradParams &p, uint32_t groups, hipStream_t s) {
   if (p.cols <= 512) return launch_kernel(norm_backward_kernel<E, CK, 64, 8, 1>, dim3(groups), dim3(512), s, p);
-  if (p.cols <= 1024) return launch_kernel(norm_backward_kernel<E, CK, 64, 8, 2>, dim3(groups), dim3(512), s, p);
+  if (p.cols <= 1024) return launch_kernel(norm_backward_kernel<E, CK, 128, 4, 1>, dim3(groups), dim3(512), s, p);
   if (p.cols <= 2048) return launch_kernel(norm_backward_kernel<E, CK, 256, 2, 1>, dim3(groups), dim3(512), s, p);
-  if (p.cols <= 4096) return launch_kernel(norm_backward_kernel<E, CK, 256, 2, 2>, dim3(groups), dim3(512), s, p);
-  if (p.cols <= 8192) return launch_kernel(norm_backward_kernel<E, CK, 512, 1, 2>, dim3(groups), dim3(512), s, p);
+  if (p.cols <= 4096) return launch_kernel(norm_backward_kernel<E, CK, 512, 1, 1>, dim3(groups), dim3(512), s, p);
+  if (p.cols <= 8192) return launch_kernel(norm_backward_kernel<E, CK, 1024, 1, 1>, dim3(groups), dim3(1024), s, p);
   return launch_kernel(norm_backward_kernel<E, CK, 1024, 1, 2>, dim3(groups), dim3(1024), s, p);
 }
 template <class E>

@@ -13,6 +13,8 @@ struct CheckpointParams {
   int32_t cols;
 };
 
+// One piece a thread (the loops are for more rows than a grid has) (8192 x 14336 bf16, us, store and load: 65.5 and 59.9; with 16 workgroups a CU that
+// walk the rows 72.2 and 71.5, with two or four rows of a thread in flight no better)
 template <class E>
 __global__ __launch_bounds__(256) void checkpoint_store_kernel(CheckpointParams p) {
   const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63)), cols32 = (p.cols + 31) & ~31;

@@ -83,6 +83,11 @@ def _check(status, what):
         raise cublaslt.CublasLtError(status, what)
 
 
+# (A call's cost on the host is what the smallest problems wait for: the structures' members and the function are looked up once.)
+def _members(p, names):
+    return [getattr(p, n) for n in names.split()]
+
+
 def checkpoint_pitches(cols):
     """(codes, scales) of a row of a checkpoint"""
     blocks = -(-cols // BLOCK)
@@ -128,12 +133,17 @@ class GatedForward(_Call):
         for name in ("gate", "up"):
             self.matrix(name, p.features, t, s.get("kept", KEPT_NONE))
         self.query(self.lib.zluda_ffn_gated_forward_workspace)
+        self._call, self._ref, self._m = self.lib.zluda_ffn_gated_forward, C.byref(p), _members(p, "x w h gate up")
 
     def run(self, x, w, h, bias=None, gate=None, gate_scales=None, up=None, up_scales=None, workspace=None, workspace_size=0, stream=None):
-        p = self.p
-        p.x.data, p.w.data, p.h.data, p.bias = x, w, h, bias
-        p.gate.data, p.gate.scales, p.up.data, p.up.scales = gate, gate_scales, up, up_scales
-        _check(self.lib.zluda_ffn_gated_forward(C.byref(p), workspace, workspace_size, stream), "zluda_ffn_gated_forward")
+        mx, mw, mh, mg, mu = self._m
+        mx.data, mw.data, mh.data, self.p.bias = x, w, h, bias
+        mg.data, mu.data = gate, up
+        if gate_scales is not None:
+            mg.scales, mu.scales = gate_scales, up_scales
+        status = self._call(self._ref, workspace, workspace_size, stream)
+        if status:
+            _check(status, "zluda_ffn_gated_forward")
 
 
 class GatedBackward(_Call):
@@ -152,14 +162,16 @@ class GatedBackward(_Call):
             getattr(p, name).data = 16 if s.get(name, default) else None
         p.dbias = 16 if s.get("bias", False) else None
         self.query(self.lib.zluda_ffn_gated_backward_workspace)
+        self._call, self._ref, self._m = self.lib.zluda_ffn_gated_backward, C.byref(p), _members(p, "dh gate up x w dx dw h dz")
 
     def run(self, dh, gate, up, x=None, w=None, dx=None, dw=None, dbias=None, h=None, dz=None, gate_scales=None, up_scales=None, x_scales=None,
             workspace=None, workspace_size=0, stream=None):
-        p = self.p
-        p.dh.data, p.gate.data, p.gate.scales, p.up.data, p.up.scales = dh, gate, gate_scales, up, up_scales
-        p.x.data, p.x.scales, p.w.data = x, x_scales, w
-        p.dx.data, p.dw.data, p.dbias, p.h.data, p.dz.data = dx, dw, dbias, h, dz
-        _check(self.lib.zluda_ffn_gated_backward(C.byref(p), workspace, workspace_size, stream), "zluda_ffn_gated_backward")
+        mdh, mg, mu, mx, mw, mdx, mdw, mh, mdz = self._m
+        mdh.data, mg.data, mg.scales, mu.data, mu.scales, mx.data, mx.scales, mw.data = dh, gate, gate_scales, up, up_scales, x, x_scales, w
+        mdx.data, mdw.data, self.p.dbias, mh.data, mdz.data = dx, dw, dbias, h, dz
+        status = self._call(self._ref, workspace, workspace_size, stream)
+        if status:
+            _check(status, "zluda_ffn_gated_backward")
 
 
 class NormForward(_Call):
@@ -171,12 +183,16 @@ class NormForward(_Call):
         self.matrix("x", p.cols, t)
         self.matrix("y", p.cols, t)
         self.matrix("kept", p.cols, t, KEPT_8BIT)
+        self._call, self._ref, self._m = self.lib.zluda_ffn_norm_forward, C.byref(p), _members(p, "x y kept")
 
     def run(self, x, y, weight=None, bias=None, mean=None, rstd=None, kept=None, kept_scales=None, stream=None):
-        p = self.p
-        p.x.data, p.y.data, p.weight, p.bias, p.mean, p.rstd = x, y, weight, bias, mean, rstd
-        p.kept.data, p.kept.scales = kept, kept_scales
-        _check(self.lib.zluda_ffn_norm_forward(C.byref(p), stream), "zluda_ffn_norm_forward")
+        p, (mx, my, mk) = self.p, self._m
+        mx.data, my.data, p.weight, p.bias, p.mean, p.rstd, mk.data = x, y, weight, bias, mean, rstd, kept
+        if kept is not None:
+            mk.scales = kept_scales
+        status = self._call(self._ref, stream)
+        if status:
+            _check(status, "zluda_ffn_norm_forward")
 
 
 class NormBackward(_Call):
@@ -190,12 +206,15 @@ class NormBackward(_Call):
             self.matrix(name, p.cols, t)
         p.dweight = p.dbias = 16 if s.get("weights", True) else None
         self.query(self.lib.zluda_ffn_norm_backward_workspace)
+        self._call, self._ref, self._m = self.lib.zluda_ffn_norm_backward, C.byref(p), _members(p, "x dy add dx")
 
     def run(self, x, dy, mean, rstd, weight=None, add=None, dx=None, dweight=None, dbias=None, x_scales=None, workspace=None, workspace_size=0, stream=None):
-        p = self.p
-        p.x.data, p.x.scales, p.dy.data, p.add.data, p.dx.data = x, x_scales, dy, add, dx
+        p, (mx, my, ma, md) = self.p, self._m
+        mx.data, mx.scales, my.data, ma.data, md.data = x, x_scales, dy, add, dx
         p.weight, p.mean, p.rstd, p.dweight, p.dbias = weight, mean, rstd, dweight, dbias
-        _check(self.lib.zluda_ffn_norm_backward(C.byref(p), workspace, workspace_size, stream), "zluda_ffn_norm_backward")
+        status = self._call(self._ref, workspace, workspace_size, stream)
+        if status:
+            _check(status, "zluda_ffn_norm_backward")
 
 
 class Checkpoint(_Call):
@@ -206,14 +225,16 @@ class Checkpoint(_Call):
         ld, lds = checkpoint_pitches(self.cols)
         self.x = _M(None, None, s.get("ldx", self.cols), 0, s["type"])
         self.c = _M(None, None, s.get("ldcodes", ld), s.get("ldscales", lds), abi.CUDA_R_8F_E4M3)
-
-    def _set(self, x, codes, scales):
-        self.x.data, self.c.data, self.c.scales = x, codes, scales
+        self._store, self._load, self._refs = self.lib.zluda_ffn_checkpoint_store, self.lib.zluda_ffn_checkpoint_load, (C.byref(self.x), C.byref(self.c))
 
     def store(self, x, codes, scales, stream=None):
-        self._set(x, codes, scales)
-        _check(self.lib.zluda_ffn_checkpoint_store(self.rows, self.cols, C.byref(self.x), C.byref(self.c), stream), "zluda_ffn_checkpoint_store")
+        self.x.data, self.c.data, self.c.scales = x, codes, scales
+        status = self._store(self.rows, self.cols, self._refs[0], self._refs[1], stream)
+        if status:
+            _check(status, "zluda_ffn_checkpoint_store")
 
     def load(self, codes, scales, x, stream=None):
-        self._set(x, codes, scales)
-        _check(self.lib.zluda_ffn_checkpoint_load(self.rows, self.cols, C.byref(self.c), C.byref(self.x), stream), "zluda_ffn_checkpoint_load")
+        self.x.data, self.c.data, self.c.scales = x, codes, scales
+        status = self._load(self.rows, self.cols, self._refs[1], self._refs[0], stream)
+        if status:
+            _check(status, "zluda_ffn_checkpoint_load")
