@@ -160,6 +160,16 @@ def test_gated_forward_many_tiles(gpu_api, t, d, f, typ, act, kept):
         check_gated(h, g, u, kept, ref, what)
 
 
+@pytest.mark.parametrize("t,d,f", [(384, 136, 14300), (2000, 200, 5601), (4000, 64, 2816)])   # 192 tokens a tile
+@pytest.mark.parametrize("typ,act,kept", [("bf16", "silu", ffn.KEPT_8BIT), ("f16", "gelu", ffn.KEPT_PLAIN)])
+def test_gated_forward_many_narrow_tiles(gpu_api, t, d, f, typ, act, kept):
+    for bias in (True, False):
+        what = "gated %s %s %d x %d x %d kept %d" % (typ, act, t, d, f, kept)
+        print(what, flush=True)
+        _, _, _, h, g, u, ref = run_gated(typ, act, t, d, f, bias, kept, seed=t)
+        check_gated(h, g, u, kept, ref, what)
+
+
 @pytest.mark.parametrize("pad,skip", [(0, 1), (1, 0), (3, 5), (8, 0), (8, 8), (4, 4)])
 @pytest.mark.parametrize("t,d,f", [(1, 128, 64), (9, 80, 72), (150, 256, 160), (520, 192, 264)])
 def test_gated_forward_pitches_and_alignments(gpu_api, t, d, f, pad, skip):

@@ -11,13 +11,13 @@ uint32_t launch_gated_bf16(const GatedParams &p, hipStream_t s);
 uint32_t launch_gated_f16(const GatedParams &p, hipStream_t s);
 
 // The tiles of the gated products: `features` x `tokens` a workgroup, its waves wp x wq, LDS stages, and the time of a stage (of
-// 64 K elements) in a full chip, us for each tile of a CU (4096 elements of K, 14336 features, 1024 tokens: 445, 309, 269, 236 us
-// for the whole call, 200 with the last, the persistent four-wave kernel; smaller tiles are less work between two barriers and read
-// more of LDS for each product).
+// 64 K elements) in a full chip, us for each tile of a CU.  From whole calls of 4096 x 14336 and 1024 tokens: 437, 304, 262, 230 us, and
+// 241 and 199 with the last two, the persistent four-wave kernel; smaller tiles are less work between two barriers and read more
+// of LDS for each product.
 struct GatedTile { int features, tokens, wp, wq, stages; float stage_us; };
-constexpr GatedTile kGatedTiles[] = {
-  {64, 32, 2, 2, 4, 0.25f}, {64, 64, 2, 2, 3, 0.345f}, {64, 128, 2, 2, 3, 0.6f}, {128, 128, 4, 2, 3, 0.93f}, {128, 256, 2, 2, 2, 1.5f}};
-constexpr int kGatedTileCount = 5, kGatedPersistent = 4;
+constexpr GatedTile kGatedTiles[] = {{64, 32, 2, 2, 4, 0.24f},   {64, 64, 2, 2, 3, 0.335f},  {64, 128, 2, 2, 3, 0.58f},
+                                     {128, 128, 4, 2, 3, 0.9f}, {128, 192, 2, 2, 2, 1.18f}, {128, 256, 2, 2, 2, 1.4f}};
+constexpr int kGatedTileCount = 6, kGatedPersistent = 4;  // (from there on)
 // in the first four of them, or (tile < 0) at any alignment
 uint32_t launch_gated_small_bf16(const GatedParams &p, int tile, hipStream_t s);
 uint32_t launch_gated_small_f16(const GatedParams &p, int tile, hipStream_t s);

@@ -13,9 +13,9 @@ template <class E>
 struct GatedMfmaParams : MfmaParams {
   GatedParams gated;
 
-  // a wave's accumulators: tiles 0 .. 3 along P are G's, 4 .. 7 U's, for features f0 .. f0 + 63; eight tiles of 16 tokens
-  template <class AccV>
-  __device__ __forceinline__ void store_tile(AccV (&acc)[8][8], int f0, int t0, const W4Staged &staged) const {
+  // a wave's accumulators: tiles 0 .. 3 along P are G's, 4 .. 7 U's, for features f0 .. f0 + 63; TQ tiles of 16 tokens
+  template <int TQ, class AccV>
+  __device__ __forceinline__ void store_tile(AccV (&acc)[8][TQ], int f0, int t0, const W4Staged &staged) const {
     const int lane = lane_here(), l4 = 4 * (lane >> 4);
     float bg[4][4], bu[4][4];
 #pragma unroll
@@ -36,7 +36,7 @@ struct GatedMfmaParams : MfmaParams {
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int b = 0; b < 8; b++) {
+    for (int b = 0; b < TQ; b++) {
       // (one column of tiles at a time, read explicitly: see w4_store_f16)
       int raw[8][4];
 #pragma unroll

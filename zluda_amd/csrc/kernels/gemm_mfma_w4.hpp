@@ -397,13 +397,15 @@ __device__ __forceinline__ void w4_store_i32(const MfmaParams &prm, AccV (&acc)[
   }
 }
 
-template <int KIND, int FQ, int FP, int EPI, class Params = MfmaParams>
+// BQ: Q indices of a tile (a gated layer also takes 192: fewer or shorter rounds where 256 leaves much of the last one empty)
+template <int KIND, int FQ, int FP, int EPI, class Params = MfmaParams, int BQ = 256>
 __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
   constexpr bool GATED = EPI == W4_EPI_GATED;
   static_assert(KIND == KIND_I8 || KIND == KIND_F8 || KIND == KIND_MXF4 || kind_is_h16(KIND), "int8, fp8, MXFP4, f16 and bf16 operands");
   constexpr bool H16 = kind_is_h16(KIND);  // v_mfma_f32_16x16x32_f16 / _bf16: the byte geometry of int8 (16 bytes of K per lane and K step)
   constexpr bool MX = KIND == KIND_MXF4;
-  constexpr int BP = 256, BQ = 256, WP = 2, WQ = 2;
+  constexpr int BP = 256, WP = 2, WQ = 2;
+  static_assert(BQ == 256 || (GATED && BQ == 192), "tile widths");
   constexpr int NWV = 4;
   constexpr int BKB = 128, CPR = 8, RPW = 8;
   constexpr int RPP = NWV * RPW;               // rows filled per DMA pass of the workgroup
@@ -414,8 +416,7 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
   constexpr int KS = KIND == KIND_F8 ? 1 : 2;  // MFMAs per fragment pair (K halves of the 128-byte stage)
   constexpr int STAGE_V4 = (BP + BQ) * CPR;    // one slot in 16-byte words: P rows, then Q rows
   constexpr int NM = HP * HQ * KS;             // MFMAs per sub-step
-  constexpr int NRD = 2 * HP;                  // ds_read_b128 per sub-step (HP == HQ)
-  static_assert(HP == HQ, "square wave tile");
+  constexpr int NRDP = 2 * HP, NRDQ = 2 * HQ;  // ds_read_b128 of a sub-step that reads P, that reads Q
   using acc_v = typename std::conditional<KIND == KIND_I8, v4i, v4f>::type;
   using frag_v = typename std::conditional<KIND != KIND_F8, v4i, v8i>::type;
   struct Frag { frag_v k[KS]; };
@@ -559,10 +560,10 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
       fragQ[par][kk] = (BP + wq * WTQ + row) * CPR + ch;
     }
   Frag pf[2][HP], qf[2][HQ];  // [half of the wave tile][fragment]
-  // ds_read_b128 number r (0 .. NRD-1) of half h of P / of Q from the slot at `so`
-  auto read_piece = [&](int so, const int (&fr)[2][2], Frag (&dst)[HP], auto h_c, auto r_c) {
-    constexpr int h = decltype(h_c)::value, r = decltype(r_c)::value;
-    constexpr int i = r / 2, kk = r % 2, tile = h * HP + i;
+  // ds_read_b128 number r (0 .. NRDP / NRDQ - 1) of half h of P / of Q from the slot at `so`
+  auto read_piece = [&](int so, const int (&fr)[2][2], auto &dst, auto h_c, auto r_c) {
+    constexpr int h = decltype(h_c)::value, r = decltype(r_c)::value, half = std::extent<std::remove_reference_t<decltype(dst)>>::value;
+    constexpr int i = r / 2, kk = r % 2, tile = h * half + i;
     const v4i x = lds[so + (tile >> 1) * 32 * CPR + fr[tile & 1][kk]];
     if constexpr (KIND == KIND_F8) {
 #pragma unroll
@@ -670,11 +671,12 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
 #endif
   };
 
-  // One sub-step: its NM MFMAs in order; behind each of the first NRD of them one fragment read (`rd(r)`), and the
+  // One sub-step: its NM MFMAs in order; behind each of the first `nr_c` of them one fragment read (`rd(r)`), and the
   // NLOAD DMA instructions spread evenly behind all of them when the sub-step refills a slot.
-  auto substep = [&](auto ph_c, auto qh_c, auto par_c, auto &&rd, auto &&extra, auto l0_c, auto l1_c, auto plain_c, int dma_dk, int dma_so,
+  auto substep = [&](auto ph_c, auto qh_c, auto par_c, auto nr_c, auto &&rd, auto &&extra, auto l0_c, auto l1_c, auto plain_c, int dma_dk, int dma_so,
                      int wave_rows) __attribute__((always_inline)) {
     constexpr int L0 = decltype(l0_c)::value, L1 = decltype(l1_c)::value;  // DMA instructions [L0, L1) of the stage ride along
+    constexpr int NRD = decltype(nr_c)::value;
     static_assert(NM >= NRD && NM >= L1 - L0, "room for the reads and the DMA of a sub-step");
     static_for<NM>([&](auto x_c) {
       constexpr int x = decltype(x_c)::value;
@@ -712,20 +714,22 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
     using Z = std::integral_constant<int, 0>;
     using LS = std::integral_constant<int, NLOAD / 2>;
     using LN = std::integral_constant<int, NLOAD>;
+    using RP = std::integral_constant<int, NRDP>;
+    using RQ = std::integral_constant<int, NRDQ>;
     auto none = [](auto) {};
     using PL = std::integral_constant<int, decltype(last_c)::value == 0 ? 1 : 0>;
     int wave_rows = wave * RPW * CPR;
 #if defined(__HIP_DEVICE_COMPILE__)
     if constexpr (MX) asm volatile("" : "+s"(wave_rows));
 #endif
-    substep(P0{}, QA{}, PAR{}, [&](auto r_c) { read_piece(so, fragQ, qf[1 - ODD], QB{}, r_c); }, none, Z{}, Z{}, PL{}, 0, 0, 0);
-    substep(P0{}, QB{}, PAR{}, [&](auto r_c) { read_piece(so, fragP, pf[1], P1{}, r_c); }, none, Z{}, Z{}, PL{}, 0, 0, 0);
+    substep(P0{}, QA{}, PAR{}, RQ{}, [&](auto r_c) { read_piece(so, fragQ, qf[1 - ODD], QB{}, r_c); }, none, Z{}, Z{}, PL{}, 0, 0, 0);
+    substep(P0{}, QB{}, PAR{}, RP{}, [&](auto r_c) { read_piece(so, fragP, pf[1], P1{}, r_c); }, none, Z{}, Z{}, PL{}, 0, 0, 0);
     // every fragment of the stage has been requested: wait for them and for this wave's share of the next stage,
     // meet the other waves; then this slot is free and the other one readable
     wait_vmcnt_barrier<0>();
     // (MXFP4: the wave's scale instruction of this stage rides behind the second MFMA, and the next stage's scales are
     // fetched behind the fragment reads of the last sub-step)
-    substep(P1{}, QB{}, PAR{}, [&](auto r_c) { read_piece(so_next, fragP, pf[0], P0{}, r_c); },
+    substep(P1{}, QB{}, PAR{}, RP{}, [&](auto r_c) { read_piece(so_next, fragP, pf[0], P0{}, r_c); },
             [&](auto x_c) {
               constexpr int x = decltype(x_c)::value;
               if constexpr (MX && LAST) {
@@ -745,12 +749,12 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
                 }
               }
             }, Z{}, LS{}, PL{}, dk, so, wave_rows);
-    substep(P1{}, QA{}, PAR{}, [&](auto r_c) { read_piece(so_next, fragQ, qf[1 - ODD], QB{}, r_c); },
+    substep(P1{}, QA{}, PAR{}, RQ{}, [&](auto r_c) { read_piece(so_next, fragQ, qf[1 - ODD], QB{}, r_c); },
             [&](auto x_c) {
               constexpr int x = decltype(x_c)::value;
-              if constexpr (MX && x == NRD - 1) scale_addr(ss + 1);
-              if constexpr (MX && x >= NRD && x < NRD + TP + TQ)
-                read_scale(std::integral_constant<int, 1 - ODD>{}, std::integral_constant<int, x - NRD>{});
+              if constexpr (MX && x == NRDQ - 1) scale_addr(ss + 1);
+              if constexpr (MX && x >= NRDQ && x < NRDQ + TP + TQ)
+                read_scale(std::integral_constant<int, 1 - ODD>{}, std::integral_constant<int, x - NRDQ>{});
             }, LS{}, LN{}, PL{}, dk, so, wave_rows);
     if constexpr (MX) ss++;
   };
@@ -761,8 +765,8 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
   };
   // the fragments a tile's first stage expects in registers (P half 0, Q half 0), from slot 0
   auto first_frags = [&]() __attribute__((always_inline)) {
-    static_for<NRD>([&](auto r_c) { read_piece(0, fragP, pf[0], P0{}, r_c); });
-    static_for<NRD>([&](auto r_c) { read_piece(0, fragQ, qf[0], P0{}, r_c); });
+    static_for<NRDP>([&](auto r_c) { read_piece(0, fragP, pf[0], P0{}, r_c); });
+    static_for<NRDQ>([&](auto r_c) { read_piece(0, fragQ, qf[0], P0{}, r_c); });
   };
   // starts the stream: the first tile's first two stages requested and landed, its first fragments in registers
   auto prime = [&]() __attribute__((always_inline)) {
@@ -881,7 +885,7 @@ __global__ __launch_bounds__(256) void gemm_mfma_w4_kernel(Params prm) {
   };
 
   // ---- the stream -------------------------------------------------------------------------------------------------
-  static_assert(!MX || NM >= NRD + TP + TQ, "room for the scale reads in a sub-step");
+  static_assert(!MX || NM >= NRDQ + TP + TQ, "room for the scale reads in a sub-step");
   prime();
   if constexpr (MX) {
     scale_addr(0);
