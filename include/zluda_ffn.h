@@ -49,7 +49,7 @@ typedef struct zluda_ffn_matrix {
 
 /* G = X Wg^T + bg, U = X Wu^T + bu, H = act(G) * U.
  * x: tokens x model, w: 2 * features x model, Wg's rows in front of Wu's, h: tokens x features, all of one 16-bit type;
- * bias: 2 * features elements of that type or NULL.  gate and up (both or neither; data == NULL: not kept) receive G and U,
+ * bias: 2 * features elements of that type or NULL; up to 2^20 features.  gate and up (both or neither; data == NULL: not kept) receive G and U,
  * in the same type or as checkpoints.  Products and sums in 32 bits; H comes from the 32-bit G and U, not from what is kept. */
 typedef struct zluda_ffn_gated {
   uint32_t activation;
@@ -82,7 +82,7 @@ uint32_t zluda_ffn_gated_backward_workspace(const zluda_ffn_gated_grad *p, size_
 /* Layer norm over rows: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(variance + eps), the variance that of the row
  * (divided by cols).  x, y: rows x cols of one type (16F, 16BF, 32F), cols up to 16384; weight, bias: cols elements of
  * weight_type (x's or 32F), NULL: 1 and 0; mean, rstd: rows floats each or NULL; kept (data == NULL: not kept): a checkpoint of
- * x, written in the same pass. */
+ * x, written in the same pass.  y may be x itself, with its pitch. */
 #define ZLUDA_FFN_NORM_MAX_COLS 16384u
 typedef struct zluda_ffn_norm {
   uint64_t rows, cols;

@@ -86,7 +86,7 @@ REFUSED = [
     ("gated_forward", forward, dict(x__data=None), IV), ("gated_forward", forward, dict(w__data=None), IV), ("gated_forward", forward, dict(h__data=None), IV),
     ("gated_forward", forward, dict(x__ld=31), IV), ("gated_forward", forward, dict(w__ld=31), IV), ("gated_forward", forward, dict(h__ld=63), IV),
     ("gated_forward", forward, dict(x__data=257), IV), ("gated_forward", forward, dict(bias=3), IV), ("gated_forward", forward, dict(gate__data=64), IV),
-    ("gated_forward", forward, dict(tokens=1 << 31), NS), ("gated_forward", forward, dict(features=1 << 31), NS),
+    ("gated_forward", forward, dict(tokens=1 << 31), NS), ("gated_forward", forward, dict(features=1 << 31), NS), ("gated_forward", forward, dict(features=(1 << 20) + 1), NS),
     ("gated_forward", forward, dict(gate__data=64, gate__type=BF, gate__ld=64, up__data=64, up__type=E4, up__ld=64, up__scales=64, up__ld_scales=2), NS),
     ("gated_forward", forward, dict(gate__data=64, gate__type=F32, gate__ld=64, up__data=64, up__type=F32, up__ld=64), NS),
     ("gated_forward", forward, dict(gate__data=64, gate__type=E4, gate__ld=64, gate__scales=1, gate__ld_scales=2, up__data=64, up__type=E4, up__ld=64, up__ld_scales=2), IV),

@@ -340,6 +340,16 @@ def test_norm_forward_pitches_and_options(gpu_api, rows, cols, pad, skip):
         assert y.guards() and c.guards() and (not keep or c.matches(x.view))
 
 
+def test_norm_forward_in_place(gpu_api):
+    for rows, cols in ((3, 100), (1000, 520), (700, 4096), (600, 9001)):
+        x, w, b, y, _, _, c, ref = run_norm("bf16", "f32", rows, cols)
+        call = ffn.NormForward(dict(type=abi.CUDA_R_16BF, weight_type=abi.CUDA_R_32F, rows=rows, cols=cols))
+        kept = Ckpt(rows, cols)
+        call.run(x=x.ptr, y=x.ptr, weight=w.ptr, bias=b.ptr, kept=kept.codes.ptr, kept_scales=kept.scales.ptr, stream=stream())
+        torch.cuda.synchronize()
+        assert torch.equal(x.view, y.view) and torch.equal(kept.codes.view, c.codes.view) and x.guards()
+
+
 def test_norm_forward_of_rows_far_from_zero_and_constant_rows(gpu_api):
     """the variance comes from differences to the mean: a mean 1000 times the spread costs no more than the bound says, and a
     constant row gives its bias"""

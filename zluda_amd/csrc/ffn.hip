@@ -15,7 +15,10 @@ using namespace zluda_amd;
 namespace {
 
 constexpr uint64_t kMaxSide = 0x7fffff00;             // sizes are 32-bit numbers inside the kernels, with room to round up
-constexpr uint64_t kGemmWorkspace = 32ull << 20;      // split-K partial tiles of the backward pass's matmuls
+constexpr uint64_t kMaxFeatures = 1 << 20;            // (2^15 blocks of 32 along a grid's second dimension)
+// Split-K partial tiles of the backward pass's matmuls.  With twice as much the planner splits further than pays here (1001 tokens, 1024 x
+// 2816: dx 24.0 us, 27.9 with 32 MiB, 29.1 with 8; 500, 4096 x 11008: 118, 122, 203).
+constexpr uint64_t kGemmWorkspace = 16ull << 20;
 constexpr int kGridY = 65535;
 
 inline bool is_h16(uint32_t type) { return type == CUDA_R_16F || type == CUDA_R_16BF; }
@@ -50,7 +53,7 @@ inline uint32_t check_vector(const void *v, uint32_t type) { return ((uintptr_t)
 // sizes of a gated layer; tokens may be 0
 uint32_t check_sizes(uint32_t activation, uint64_t tokens, uint64_t features, uint64_t model) {
   if (activation > ZLUDA_FFN_RELU || !features || !model) return CUBLAS_STATUS_INVALID_VALUE;
-  return tokens > kMaxSide || features > kMaxSide / 2 || model > kMaxSide ? CUBLAS_STATUS_NOT_SUPPORTED : CUBLAS_STATUS_SUCCESS;
+  return tokens > kMaxSide || features > kMaxFeatures || model > kMaxSide ? CUBLAS_STATUS_NOT_SUPPORTED : CUBLAS_STATUS_SUCCESS;
 }
 
 uint32_t check_forward(const zluda_ffn_gated *p) {

@@ -28,7 +28,7 @@ inline uint32_t launch_gated_small(const GatedParams &p, int tile, hipStream_t s
   case 1: return launch_gated_tile<E, 1>(p, s);
   case 2: return launch_gated_tile<E, 2>(p, s);
   case 3: return launch_gated_tile<E, 3>(p, s);
-  default: return launch_kernel(gated_any_kernel<E>, dim3((p.features + 31) / 32, (p.tokens + 63) / 64), dim3(256), s, p);
+  default: return launch_kernel(gated_any_kernel<E>, dim3((p.tokens + 63) / 64, (p.features + 31) / 32), dim3(256), s, p);
   }
 }
 

@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void gated_any_kernel(GatedParams p) {
   constexpr int PITCH = 5;  // 16-byte words of a row: four and a pad
   __shared__ ffn_u4 lw[64 * PITCH], lx[64 * PITCH];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6, r16 = lane & 15, grp = lane >> 4;
-  const int f0 = blockIdx.x * 32, t0 = blockIdx.y * 64;
+  const int f0 = blockIdx.y * 32, t0 = blockIdx.x * 64;
   // the row and the eight K elements that this thread brings: rows past the end repeat the last one, their results are dropped
   const int row = t >> 2, kc = (t & 3) * 8;
   const int f = min(f0 + (row & 31), p.features - 1) + (row < 32 ? 0 : p.features);

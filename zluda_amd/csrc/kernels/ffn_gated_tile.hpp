@@ -25,11 +25,12 @@ struct GatedTileParams : MfmaParams {
 template <class E, int BF, int BT, int WP, int WQ, int NS>
 __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams prm) {
   using raw = typename E::raw;
-  constexpr int NW = WP * WQ, RPP = 8 * NW;           // rows a DMA pass of the workgroup fills
-  constexpr int BP = 2 * BF, LP = BP / RPP, LQ = BT / RPP, NLOAD = LP + LQ;
+  constexpr int BP = 2 * BF;
+  constexpr PipeCounts PC = pipe_counts(false, BP, BT, WP, WQ, 128, NS);
+  constexpr int RPP = PC.rpp, LP = PC.lp, LQ = PC.lq, NLOAD = PC.nload;  // rows a DMA pass of the workgroup fills, instructions a stage
   constexpr int FW = BF / WP, TG = FW / 16, TQ = BT / WQ / 16;  // a wave's share
   constexpr int STAGE = (BP + BT) * 8;                // one slot in 16-byte words
-  static_assert(BP % RPP == 0 && BT % RPP == 0 && FW % 32 == 0 && BT % (16 * WQ) == 0, "whole passes, whole pairs of tiles");
+  static_assert(RPP % 32 == 0 && BP % RPP == 0 && BT % RPP == 0 && FW % 32 == 0 && BT % (16 * WQ) == 0, "whole passes, whole pairs of tiles");
   static_assert(NS * STAGE * 16 <= 160 * 1024 && (NS - 1) * NLOAD < 64, "LDS and vmcnt");
   __shared__ v4i lds[NS * STAGE];
 
@@ -42,21 +43,16 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
   // ---- DMA: lane l -> row l / 8 of the eight an instruction fills, chunk l % 8 -------------------------------------------------
   const __amdgpu_buffer_rsrc_t rw = __builtin_amdgcn_make_buffer_rsrc((void *)p.w, 0, 0x80000000, 0x00020000);
   const __amdgpu_buffer_rsrc_t rx = __builtin_amdgcn_make_buffer_rsrc((void *)p.x, 0, 0x80000000, 0x00020000);
-  const int drow = wave * 8 + (lane >> 3), dchunk = ((lane & 7) ^ swz(drow)) * 16;  // (passes are 16 rows apart at least: see below)
-  int ow[LP], ox[LQ], cw[LP], cx[LQ];
+  const int drow = wave * 8 + (lane >> 3), dchunk = ((lane & 7) ^ swz(drow)) * 16;  // (passes are a multiple of 32 rows apart: same swizzle)
+  int ow[LP], ox[LQ];
 #pragma unroll
   for (int i = 0; i < LP; i++) {
     const int r = drow + RPP * i, j = r % (2 * FW);
     const int f = min(f0 + r / (2 * FW) * FW + j % FW, p.features - 1) + (j < FW ? 0 : p.features);
-    cw[i] = RPP % 32 ? ((lane & 7) ^ swz(r)) * 16 : dchunk;
-    ow[i] = f * (int)p.ldw * 2 + cw[i];
+    ow[i] = f * (int)p.ldw * 2 + dchunk;
   }
 #pragma unroll
-  for (int i = 0; i < LQ; i++) {
-    const int r = drow + RPP * i;
-    cx[i] = RPP % 32 ? ((lane & 7) ^ swz(BP + r)) * 16 : ((lane & 7) ^ swz(drow)) * 16;
-    ox[i] = min(t0 + r, p.tokens - 1) * (int)p.ldx * 2 + cx[i];
-  }
+  for (int i = 0; i < LQ; i++) ox[i] = min(t0 + drow + RPP * i, p.tokens - 1) * (int)p.ldx * 2 + dchunk;
   const int kbytes = p.model * 2, stages = (kbytes + 127) / 128;
   // Tiles start their walk along K three stages apart and wrap round.  All starting at K = 0, they would read the same few
   // columns of W at a time, and rows a power of two apart share memory channels (one token, 4096 x 14336: 50.6 -> 42.7 us; rows of
@@ -66,8 +62,8 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
     constexpr int i = decltype(i_c)::value;
     const int at = (kt + turn < stages ? kt + turn : kt + turn - stages) * 128, live = kt < stages ? -1 : 0;  // (past the end: every lane the matrix's first bytes)
     v4i *base = &lds[slot * STAGE + wave * 64];
-    if constexpr (i < LP) lds_dma16(rw, base + RPP * 8 * i, (ow[i] | (at + cw[i] < kbytes ? 0 : (int)0x80000000)) & live, at & live);
-    else lds_dma16(rx, base + BP * 8 + RPP * 8 * (i - LP), (ox[i - LP] | (at + cx[i - LP] < kbytes ? 0 : (int)0x80000000)) & live, at & live);
+    if constexpr (i < LP) lds_dma16(rw, base + RPP * 8 * i, (ow[i] | (at + dchunk < kbytes ? 0 : (int)0x80000000)) & live, at & live);
+    else lds_dma16(rx, base + BP * 8 + RPP * 8 * (i - LP), (ox[i - LP] | (at + dchunk < kbytes ? 0 : (int)0x80000000)) & live, at & live);
   };
 
   v4f acc[2 * TG][TQ];
@@ -93,14 +89,14 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
     fr[cur][h][i] = __builtin_bit_cast(ffn_u4, lds[slot * STAGE + (i < 2 * TG ? at_w : at_x)[h][tile & 1] + (tile >> 1) * 256]);
   };
   static_for<NS>([&](auto st_c) { static_for<NLOAD>([&](auto i_c) { issue(i_c, decltype(st_c)::value, decltype(st_c)::value); }); });
-  wait_vmcnt_barrier<(NS - 1) * NLOAD>();
+  wait_vmcnt_barrier<PC.wait_prologue>();
   static_for<NR>([&](auto r_c) { read(r_c, std::integral_constant<int, 0>{}, 0); });
   int slot = 0;
   auto do_stage = [&](auto cur_c, int kt) __attribute__((always_inline)) {
     constexpr int cur = decltype(cur_c)::value;
     using Next = std::integral_constant<int, 1 - cur>;
     const int next = slot == NS - 1 ? 0 : slot + 1;
-    wait_vmcnt_barrier<(NS - 2) * NLOAD>();
+    wait_vmcnt_barrier<PC.wait_stage>();
     __builtin_amdgcn_sched_barrier(0);
     // the reads behind the first five eighths of the MFMAs, the DMA behind the rest
     constexpr int HR = NM * 5 / 8 > 0 ? NM * 5 / 8 : 1, HD = NM - HR > 0 ? NM - HR : 1;
