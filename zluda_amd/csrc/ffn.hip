@@ -89,16 +89,20 @@ uint32_t grad_shares(uint64_t tokens, uint64_t features, bool sums) {
   return (uint32_t)std::min<uint64_t>({want, most, kGridY});
 }
 
+// Rows of the workspace's matrices start on cache lines (128 bytes): elsewhere each piece of a row that the matmuls fetch touches two
+// (forward products, 603 tokens, 8608 features: model 3520 87 us, 3496 109).
+int64_t aligned_pitch(uint64_t cols) { return (int64_t)((cols + 63) & ~63ull); }
+
 GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
   GradPlan g;
   memset(&g, 0, sizeof(g));
   uint64_t at = 0;
-  g.lddz = p->dz.data ? p->dz.ld : (int64_t)((2 * p->features + 7) & ~7ull);
+  g.lddz = p->dz.data ? p->dz.ld : aligned_pitch(2 * p->features);
   g.shares = grad_shares(p->tokens, p->features, p->dbias != nullptr);
   g.dz = at;
   if (!p->dz.data) at += aligned256(p->tokens * (uint64_t)g.lddz * 2);
   g.x = at;
-  if (p->dw.data && p->x.type == CUDA_R_8F_E4M3) at += aligned256(p->tokens * ((p->model + 7) & ~7ull) * 2);
+  if (p->dw.data && p->x.type == CUDA_R_8F_E4M3) at += aligned256(p->tokens * (uint64_t)aligned_pitch(p->model) * 2);
   g.sums = at;
   if (p->dbias) at += aligned256((uint64_t)g.shares * 2 * p->features * 4);
   g.gemm = at;
@@ -156,7 +160,7 @@ uint32_t checkpoint_call(bool store, uint64_t rows, uint64_t cols, const zluda_f
 
 template <class E, bool CK>
 uint32_t launch_gated_grad(const GatedGradParams &g, uint32_t shares, hipStream_t s) {
-  const dim3 grid((g.features + 511) / 512, shares);
+  const dim3 grid((g.features + 511) / 512 + (g.load.x ? (g.load.cols + 511) / 512 : 0), shares);
   switch (g.activation) {
   case ZLUDA_FFN_SILU: return launch_kernel(gated_grad_kernel<E, CK, 0>, grid, dim3(256), s, g);
   case ZLUDA_FFN_GELU: return launch_kernel(gated_grad_kernel<E, CK, 1>, grid, dim3(256), s, g);
@@ -215,11 +219,12 @@ uint32_t launch_norm(const NormParams &p, hipStream_t s) {
 }
 
 // Rows a workgroup of the gradient kernel takes at a time, and workgroups: two a CU (one of 1024 threads), each with at least two
-// rounds of rows, because every workgroup's partial sums are written and read again (us with at least 1, 2, 4, 8 rounds: 300 x 4096
-// bf16 12.2, 10.6, 11.1, 13.3; 777 x 1001 f16 10.1, 10.0, 11.5, 16.2; 500 x 16384 50.1, 35.2, 29.1, 35.0)
+// rounds of rows where there are more than 64 rounds, because every workgroup's partial sums are written and read again (us with at
+// least 1, 2, 4 rounds: 300 x 4096 bf16 12.2, 10.6, 11.1; 777 x 1001 f16 10.1, 10.0, 11.5; 400 x 16384 32.6, 29.1, 30.8; 62 x 9353 13.7,
+// 16.1, 21.8; 3 x 10216 11.1, 13.3, 15.8)
 int norm_grad_rows_each(uint64_t cols) { return cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1; }
 uint32_t norm_grad_groups(uint64_t rows, uint64_t cols) {
-  const int least = norm_grad_rows_each(cols) * (cols <= 8192 ? 2 : 4);
+  const int each = norm_grad_rows_each(cols), least = rows <= 64ull * each ? each : 2 * each;
   return (uint32_t)std::min<uint64_t>((rows + least - 1) / least, (uint64_t)cus() * (cols <= 4096 ? 2 : 1));
 }
 
@@ -313,6 +318,12 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
   g.features = (int32_t)p->features;
   g.activation = p->activation;
   const bool ck = p->gate.type == CUDA_R_8F_E4M3;
+  // a checkpoint of x is decoded for the product by the same launch
+  zluda_ffn_matrix x = p->x;
+  if (p->dw.data && p->x.type == CUDA_R_8F_E4M3) {
+    x = {ws + plan.x, nullptr, aligned_pitch(p->model), 0, type};
+    g.load = CheckpointParams{x.data, (uint8_t *)p->x.data, (uint8_t *)p->x.scales, (int64_t)p->tokens, x.ld, p->x.ld, p->x.ld_scales, (int32_t)p->model};
+  }
   FFN_CHECK(type == CUDA_R_16BF ? (ck ? launch_gated_grad<ElemBF16, true>(g, plan.shares, s) : launch_gated_grad<ElemBF16, false>(g, plan.shares, s))
                                 : (ck ? launch_gated_grad<ElemF16, true>(g, plan.shares, s) : launch_gated_grad<ElemF16, false>(g, plan.shares, s)));
   if (p->dbias) {
@@ -325,11 +336,6 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
   if (p->dx.data)
     FFN_CHECK(run_matmul(type, CUBLAS_OP_N, CUBLAS_OP_N, p->model, p->tokens, f2, p->w.data, p->w.ld, g.dz, plan.lddz, p->dx.data, p->dx.ld, gemm_ws, kGemmWorkspace, s));
   if (p->dw.data) {
-    zluda_ffn_matrix x = p->x;
-    if (p->x.type == CUDA_R_8F_E4M3) {
-      x = {ws + plan.x, nullptr, (int64_t)((p->model + 7) & ~7ull), 0, type};
-      FFN_CHECK(run_checkpoint(false, p->tokens, p->model, x, p->x, s));
-    }
     FFN_CHECK(run_matmul(type, CUBLAS_OP_N, CUBLAS_OP_T, p->model, f2, p->tokens, x.data, x.ld, g.dz, plan.lddz, p->dw.data, p->dw.ld, gemm_ws, kGemmWorkspace, s));
   }
   return CUBLAS_STATUS_SUCCESS;

@@ -28,14 +28,19 @@ __global__ __launch_bounds__(256) void checkpoint_store_kernel(CheckpointParams 
 }
 
 template <class E>
-__global__ __launch_bounds__(256) void checkpoint_load_kernel(CheckpointParams p) {
-  const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63));
+__device__ __forceinline__ void checkpoint_load(const CheckpointParams &p, int strip) {
+  const int col = 8 * (strip * 64 + (threadIdx.x & 63));
   if (col >= p.cols) return;
   for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < p.rows; row += gridDim.y * 4) {
     float v[8];
     ckpt_get8(ckpt_load8(p.codes + row * p.ld_codes, p.scales + row * p.ld_scales, col), v);
     store8<E>((typename E::raw *)p.x + row * p.ldx + col, v, p.cols - col);
   }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void checkpoint_load_kernel(CheckpointParams p) {
+  checkpoint_load<E>(p, blockIdx.x);
 }
 
 struct GatedGradParams {
@@ -46,12 +51,18 @@ struct GatedGradParams {
   int64_t tokens, lddh, ldg, ldu, ldgs, ldus, lddz, ldh;
   int32_t features;
   uint32_t activation;
+  CheckpointParams load;                   // a checkpoint to decode beside it: the workgroups behind the features' strips; x == NULL: none
 };
 
 // dU = dH act(G), dG = dH U act'(G); H = act(G) U on request.  CK: gate and up are checkpoints.
 template <class E, bool CK, int ACT>
 __global__ __launch_bounds__(256) void gated_grad_kernel(GatedGradParams p) {
   using raw = typename E::raw;
+  const int strips = (p.features + 511) / 512;
+  if ((int)blockIdx.x >= strips) {
+    checkpoint_load<E>(p.load, blockIdx.x - strips);
+    return;
+  }
   const int lane = threadIdx.x & 63, phase = threadIdx.x >> 6, col = 8 * (blockIdx.x * 64 + lane), n = p.features - col;
   float sg[8], su[8];
 #pragma unroll
