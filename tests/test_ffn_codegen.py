@@ -41,14 +41,22 @@ def test_a_stage_is_read_only_after_it_has_landed(features, tokens, wp, wq, ring
     """replays a wave's issue order: all of a ring's stages, then a wait and the reads of the next stage in front of each refill;
     loads retire in order, so a wait for at most n outstanding has everything but the youngest n"""
     loads = (2 * features + tokens) // (8 * wp * wq)
-    for stages in (1, 2, 3, 5, 16):
-        issued = [s for s in range(ring) for _ in range(loads)]
-        landed = issued[:len(issued) - (ring - 1) * loads]
-        assert landed.count(0) == loads                                     # the prologue's wait
+    for stages in (1, 2, 3, 4, 5, 6, 7, 16, 17):
+        issued = [s for s in range(min(ring, stages)) for _ in range(loads)]
+
+        def landed(younger):
+            """the wait of wait_for(younger): at most that many stages' instructions outstanding"""
+            n = (ring - 1 if younger >= ring - 1 else ring - 2 if younger == ring - 2 else 1 if ring > 3 and younger == 1 else 0) * loads
+            return issued[:len(issued) - n] if n else issued
+
+        assert landed(stages - 1).count(0) == loads                         # the prologue's wait
         for kt in range(stages):
-            landed = issued[:len(issued) - (ring - 2) * loads]
-            assert landed.count(kt + 1) == loads                            # read behind this barrier
-            issued += [kt + ring] * loads                                   # into the slot of stage kt, whose fragments are in registers
+            done = landed(ring - 2 if kt + ring < stages else min(stages - kt, ring) - 2)
+            if kt + 1 < stages:
+                assert done.count(kt + 1) == loads                          # read behind this barrier
+            if kt + ring < stages:
+                issued += [kt + ring] * loads                               # into the slot of stage kt, whose fragments are in registers
+        assert issued == [s for s in range(stages) for _ in range(loads)]
     assert (ring - 1) * loads < 64 and ring * (2 * features + tokens) * 128 <= 160 * 1024
 
 

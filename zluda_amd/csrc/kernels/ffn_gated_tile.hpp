@@ -8,8 +8,8 @@
 // slots in LDS; rows are eight 16-byte chunks, XOR-swizzled as in gemm_mfma.hpp.  The fragments of a stage are read from LDS behind
 // the products of the stage before it, so a wave waits neither for memory nor for LDS once it runs.  One barrier a stage: behind
 // it stage kt + 1 has landed for every wave and every wave holds its fragments of stage kt, whose slot takes stage kt + NS.  The waits
-// count the instructions of the younger stages (mfma_wait_counts.hpp has the rule: loads retire in order unless all their lanes are
-// out of range, so stages past the end of K are real loads of one cache line, and a K tail holds its row's first chunk).
+// count the instructions of the younger stages (mfma_wait_counts.hpp has the rule: loads that make a round trip to memory retire in
+// order; a K tail holds its row's first chunk).  Nothing is requested behind the end of K, and the last waits count what is left.
 //
 // LDS rows of W: for each of the WP wave rows its FW gate rows, then its FW up rows.
 #pragma once
@@ -60,10 +60,10 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
   const int turn = item.p * 3 % stages;
   auto issue = [&](auto i_c, int kt, int slot) __attribute__((always_inline)) {  // instruction i of a stage
     constexpr int i = decltype(i_c)::value;
-    const int at = (kt + turn < stages ? kt + turn : kt + turn - stages) * 128, live = kt < stages ? -1 : 0;  // (past the end: every lane the matrix's first bytes)
+    const int at = (kt + turn < stages ? kt + turn : kt + turn - stages) * 128, oob = at + dchunk < kbytes ? 0 : (int)0x80000000;
     v4i *base = &lds[slot * STAGE + wave * 64];
-    if constexpr (i < LP) lds_dma16(rw, base + RPP * 8 * i, (ow[i] | (at + dchunk < kbytes ? 0 : (int)0x80000000)) & live, at & live);
-    else lds_dma16(rx, base + BP * 8 + RPP * 8 * (i - LP), (ox[i - LP] | (at + dchunk < kbytes ? 0 : (int)0x80000000)) & live, at & live);
+    if constexpr (i < LP) lds_dma16(rw, base + RPP * 8 * i, ow[i] | oob, at);
+    else lds_dma16(rx, base + BP * 8 + RPP * 8 * (i - LP), ox[i - LP] | oob, at);
   };
 
   v4f acc[2 * TG][TQ];
@@ -88,15 +88,27 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
     constexpr int tile = i < 2 * TG ? i : i - 2 * TG;
     fr[cur][h][i] = __builtin_bit_cast(ffn_u4, lds[slot * STAGE + (i < 2 * TG ? at_w : at_x)[h][tile & 1] + (tile >> 1) * 256]);
   };
-  static_for<NS>([&](auto st_c) { static_for<NLOAD>([&](auto i_c) { issue(i_c, decltype(st_c)::value, decltype(st_c)::value); }); });
-  wait_vmcnt_barrier<PC.wait_prologue>();
+  // waits until at most `younger` stages of this wave's instructions are outstanding
+  auto wait_for = [&](int younger) __attribute__((always_inline)) {
+    if (younger >= NS - 1) wait_vmcnt_barrier<(NS - 1) * NLOAD>();
+    else if (younger == NS - 2) wait_vmcnt_barrier<(NS - 2) * NLOAD>();
+    else if (NS > 3 && younger == 1) wait_vmcnt_barrier<NLOAD>();
+    else wait_vmcnt_barrier<0>();
+  };
+  static_assert(PC.wait_prologue == (NS - 1) * NLOAD && PC.wait_stage == (NS - 2) * NLOAD && NS <= 4, "counts");
+  static_for<NS>([&](auto st_c) {
+    if (decltype(st_c)::value < stages) static_for<NLOAD>([&](auto i_c) { issue(i_c, decltype(st_c)::value, decltype(st_c)::value); });
+  });
+  wait_for(stages - 1);
   static_for<NR>([&](auto r_c) { read(r_c, std::integral_constant<int, 0>{}, 0); });
   int slot = 0;
-  auto do_stage = [&](auto cur_c, int kt) __attribute__((always_inline)) {
+  auto do_stage = [&](auto cur_c, auto refill_c, int kt) __attribute__((always_inline)) {
     constexpr int cur = decltype(cur_c)::value;
+    constexpr bool REFILL = decltype(refill_c)::value != 0;  // stage kt + NS exists
     using Next = std::integral_constant<int, 1 - cur>;
     const int next = slot == NS - 1 ? 0 : slot + 1;
-    wait_vmcnt_barrier<PC.wait_stage>();
+    if constexpr (REFILL) wait_vmcnt_barrier<PC.wait_stage>();
+    else wait_for(min(stages - kt, NS) - 2);
     __builtin_amdgcn_sched_barrier(0);
     // the reads behind the first five eighths of the MFMAs, the DMA behind the rest
     constexpr int HR = NM * 5 / 8 > 0 ? NM * 5 / 8 : 1, HD = NM - HR > 0 ? NM - HR : 1;
@@ -105,19 +117,26 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
       ffn_mfma<E>(fr[cur][h][a], fr[cur][h][2 * TG + b], acc[a][b]);
       constexpr int r0 = x < HR ? NR * x / HR : NR, r1 = x < HR ? NR * (x + 1) / HR : NR;
       static_for<r1 - r0>([&](auto r_c) { read(std::integral_constant<int, r0 + decltype(r_c)::value>{}, Next{}, next); });
-      constexpr int d0 = x < HR ? 0 : NLOAD * (x - HR) / HD, d1 = x < HR ? 0 : NLOAD * (x - HR + 1) / HD;
+      constexpr int d0 = x < HR || !REFILL ? 0 : NLOAD * (x - HR) / HD, d1 = x < HR || !REFILL ? 0 : NLOAD * (x - HR + 1) / HD;
       static_for<d1 - d0>([&](auto i_c) { issue(std::integral_constant<int, d0 + decltype(i_c)::value>{}, kt + NS, slot); });
       __builtin_amdgcn_sched_barrier(0);
     });
     slot = next;
   };
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
   int kt = 0;
-  for (; kt + 1 < stages; kt += 2) {
-    do_stage(std::integral_constant<int, 0>{}, kt);
-    do_stage(std::integral_constant<int, 1>{}, kt + 1);
+  for (; kt + 1 + NS < stages; kt += 2) {
+    do_stage(C0{}, C1{}, kt);
+    do_stage(C1{}, C1{}, kt + 1);
   }
-  if (kt < stages) do_stage(std::integral_constant<int, 0>{}, kt);
-  __builtin_amdgcn_s_waitcnt(0);  // (nothing may land in LDS that the next workgroup owns)
+  if (kt + NS < stages) do_stage(C0{}, C1{}, kt++);
+  if (kt & 1) do_stage(C1{}, C0{}, kt++);
+  for (; kt + 1 < stages; kt += 2) {
+    do_stage(C0{}, C0{}, kt);
+    do_stage(C1{}, C0{}, kt + 1);
+  }
+  if (kt < stages) do_stage(C0{}, C0{}, kt);
 
   const int fw = f0 + wp * FW;
   float bg[TG][4], bu[TG][4];
