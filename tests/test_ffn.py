@@ -128,7 +128,9 @@ def test_null_structures_and_small_workspaces():
     assert lib.zluda_ffn_gated_backward(C.byref(p), 1 << 20, n.value - 1, None) == NOMEM
     assert lib.zluda_ffn_gated_backward(C.byref(p), None, n.value, None) == NOMEM
     assert lib.zluda_ffn_gated_backward(C.byref(p), (1 << 20) + 8, n.value, None) == IV
-    q = norm_grad()
+    q = norm_grad(rows=1)
+    assert lib.zluda_ffn_norm_backward_workspace(C.byref(q), C.byref(n)) == 0 and n.value == 0      # one workgroup: no partial sums
+    q = norm_grad(rows=4000)
     assert lib.zluda_ffn_norm_backward_workspace(C.byref(q), C.byref(n)) == 0 and n.value >= 2 * 64 * 4
     assert lib.zluda_ffn_norm_backward(C.byref(q), 1 << 20, n.value - 1, None) == NOMEM
     M = ffn.zluda_ffn_matrix

@@ -225,6 +225,7 @@ uint32_t launch_norm(const NormParams &p, hipStream_t s) {
 int norm_grad_rows_each(uint64_t cols) { return cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1; }
 uint32_t norm_grad_groups(uint64_t rows, uint64_t cols) {
   const int each = norm_grad_rows_each(cols), least = rows <= 64ull * each ? each : 2 * each;
+  if (rows <= 3ull * each) return 1;  // (the sums are its own: no second launch; 2 x 3000 5.2 us, 7.1 by way of partial sums, 4 x 3000 7.8 and 6.9)
   return (uint32_t)std::min<uint64_t>((rows + least - 1) / least, (uint64_t)cus() * (cols <= 4096 ? 2 : 1));
 }
 
@@ -368,7 +369,8 @@ extern "C" uint32_t zluda_ffn_norm_forward(const zluda_ffn_norm *p, void *stream
 extern "C" uint32_t zluda_ffn_norm_backward_workspace(const zluda_ffn_norm_grad *p, size_t *bytes) {
   if (!p || !bytes || !p->cols) return CUBLAS_STATUS_INVALID_VALUE;
   if (p->cols > ZLUDA_FFN_NORM_MAX_COLS) return CUBLAS_STATUS_NOT_SUPPORTED;
-  *bytes = p->dweight ? (size_t)norm_grad_groups(p->rows, p->cols) * 2 * p->cols * 4 : 0;
+  const uint32_t groups = p->rows ? norm_grad_groups(p->rows, p->cols) : 1;
+  *bytes = p->dweight && groups > 1 ? (size_t)groups * 2 * p->cols * 4 : 0;  // (a single workgroup has the sums themselves)
   return CUBLAS_STATUS_SUCCESS;
 }
 
@@ -388,13 +390,13 @@ extern "C" uint32_t zluda_ffn_norm_backward(const zluda_ffn_norm_grad *p, void *
     return CUBLAS_STATUS_SUCCESS;
   }
   const uint32_t groups = norm_grad_groups(p->rows, p->cols);
-  NormGradParams n{p->x.data, p->dy.data, p->add.data, (const uint8_t *)p->x.scales, p->dx.data, p->weight, p->mean, p->rstd, p->dweight ? (float *)workspace : nullptr,
-                   (int64_t)p->rows, p->x.ld, p->x.ld_scales, p->dy.ld, p->add.ld, p->dx.ld, (int32_t)p->cols, p->weight_type};
+  NormGradParams n{p->x.data, p->dy.data, p->add.data, (const uint8_t *)p->x.scales, p->dx.data, p->weight, p->mean, p->rstd, p->dweight && groups > 1 ? (float *)workspace : nullptr,
+                   groups > 1 ? nullptr : p->dweight, groups > 1 ? nullptr : p->dbias, (int64_t)p->rows, p->x.ld, p->x.ld_scales, p->dy.ld, p->add.ld, p->dx.ld, (int32_t)p->cols, p->weight_type};
   const bool ck = p->x.type == CUDA_R_8F_E4M3;
   FFN_CHECK(p->dy.type == CUDA_R_16BF  ? launch_norm_grad<ElemBF16>(n, ck, groups, s)
             : p->dy.type == CUDA_R_16F ? launch_norm_grad<ElemF16>(n, ck, groups, s)
                                        : launch_norm_grad<ElemF32>(n, ck, groups, s));
-  if (!p->dweight) return CUBLAS_STATUS_SUCCESS;
+  if (!p->dweight || groups == 1) return CUBLAS_STATUS_SUCCESS;
   NormFinishParams f{n.part, p->dweight, p->dbias, (int32_t)groups, (int32_t)p->cols, p->weight_type};
   return launch_kernel(norm_finish_kernel<16, 64>, dim3((uint32_t)((p->cols + 15) / 16), 2), dim3(1024), s, f);
 }

@@ -73,15 +73,16 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
     for (int b = 0; b < TQ; b++) acc[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
   constexpr int NR = 2 * (2 * TG + TQ), NM = 2 * 2 * TG * TQ;  // fragment reads and MFMAs of a stage
   ffn_u4 fr[2][2][2 * TG + TQ];                               // [stage parity][half of the stage][W tiles, X tiles]
-  // word of a fragment inside a slot: tiles are 16 rows apart and the swizzle repeats after 32
+  // Word of a fragment inside a slot: tiles are 16 rows apart and the swizzle repeats after 32.  A lane group's two pieces of a stage are
+  // neighbours (any K order will do that is the same for W and X): so no part of a ds_read_b128 meets a bank conflict.
   int at_w[2][2], at_x[2][2];  // [half][tile parity]
 #pragma unroll
   for (int h = 0; h < 2; h++)
 #pragma unroll
     for (int par = 0; par < 2; par++) {
       const int rp = wp * 2 * FW + 16 * par + r16, rq = BP + wq * (16 * TQ) + 16 * par + r16;
-      at_w[h][par] = rp * 8 + ((4 * h + grp) ^ swz(rp));
-      at_x[h][par] = rq * 8 + ((4 * h + grp) ^ swz(rq));
+      at_w[h][par] = rp * 8 + ((2 * grp + h) ^ swz(rp));
+      at_x[h][par] = rq * 8 + ((2 * grp + h) ^ swz(rq));
     }
   auto read = [&](auto r_c, auto cur_c, int slot) __attribute__((always_inline)) {  // fragment read r of a stage
     constexpr int r = decltype(r_c)::value, h = r / (2 * TG + TQ), i = r % (2 * TG + TQ), cur = decltype(cur_c)::value;
@@ -110,14 +111,14 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
     if constexpr (REFILL) wait_vmcnt_barrier<PC.wait_stage>();
     else wait_for(min(stages - kt, NS) - 2);
     __builtin_amdgcn_sched_barrier(0);
-    // the reads behind the first five eighths of the MFMAs, the DMA behind the rest
-    constexpr int HR = NM * 5 / 8 > 0 ? NM * 5 / 8 : 1, HD = NM - HR > 0 ? NM - HR : 1;
+    // the reads and the DMA spread over all of the MFMAs (reads first, then the DMA: up to 7 % slower, 100 tokens, 2048 x 5632 16.1 against
+    // 14.9 us; a stage's requests set out earlier)
     static_for<NM>([&](auto x_c) {
       constexpr int x = decltype(x_c)::value, h = x / (2 * TG * TQ), a = x % (2 * TG * TQ) / TQ, b = x % TQ;
       ffn_mfma<E>(fr[cur][h][a], fr[cur][h][2 * TG + b], acc[a][b]);
-      constexpr int r0 = x < HR ? NR * x / HR : NR, r1 = x < HR ? NR * (x + 1) / HR : NR;
+      constexpr int r0 = NR * x / NM, r1 = NR * (x + 1) / NM;
       static_for<r1 - r0>([&](auto r_c) { read(std::integral_constant<int, r0 + decltype(r_c)::value>{}, Next{}, next); });
-      constexpr int d0 = x < HR || !REFILL ? 0 : NLOAD * (x - HR) / HD, d1 = x < HR || !REFILL ? 0 : NLOAD * (x - HR + 1) / HD;
+      constexpr int d0 = REFILL ? NLOAD * x / NM : 0, d1 = REFILL ? NLOAD * (x + 1) / NM : 0;
       static_for<d1 - d0>([&](auto i_c) { issue(std::integral_constant<int, d0 + decltype(i_c)::value>{}, kt + NS, slot); });
       __builtin_amdgcn_sched_barrier(0);
     });

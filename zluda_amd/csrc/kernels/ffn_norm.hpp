@@ -29,7 +29,8 @@ struct NormGradParams {
   void *dx;                  // or NULL
   const void *weight;        // or NULL
   const float *mean, *rstd;
-  float *part;               // [2][gridDim.x][cols]: partial sums of dweight, of dbias; NULL: not wanted
+  float *part;               // [2][gridDim.x][cols]: partial sums of dweight, of dbias; NULL: not wanted, or
+  void *dweight, *dbias;     // the sums themselves, of a single workgroup; NULL: not wanted, or by way of `part`
   int64_t rows, ldx, ld_scales, lddy, ldadd, lddx;
   int32_t cols;
   uint32_t weight_type;
@@ -244,14 +245,23 @@ __global__ __launch_bounds__(T *R) void norm_backward_kernel(NormGradParams p) {
       }
     }
   }
-  if (!p.part) return;
+  if (!p.part && !p.dweight) return;
   float *part_w = p.part + (int64_t)blockIdx.x * p.cols, *part_b = p.part + ((int64_t)gridDim.x + blockIdx.x) * p.cols;
 #pragma unroll
   for (int i = 0; i < NV; i++) {
     const int col = 8 * (lane + T * i);
     if constexpr (R == 1) {
-      store8<ElemF32>(part_w + col, dw[i], p.cols - col);
-      store8<ElemF32>(part_b + col, db[i], p.cols - col);
+      const int n = p.cols - col;
+      if (p.part) {
+        store8<ElemF32>(part_w + col, dw[i], n);
+        store8<ElemF32>(part_b + col, db[i], n);
+      } else if (p.weight_type == CUDA_R_32F) {
+        store8<ElemF32>((float *)p.dweight + col, dw[i], n);
+        store8<ElemF32>((float *)p.dbias + col, db[i], n);
+      } else {
+        store8<E>((typename E::raw *)p.dweight + col, dw[i], n);
+        store8<E>((typename E::raw *)p.dbias + col, db[i], n);
+      }
     } else {
       // the groups' sums meet in LDS, group after group
 #pragma unroll
@@ -265,7 +275,9 @@ __global__ __launch_bounds__(T *R) void norm_backward_kernel(NormGradParams p) {
 #pragma unroll
           for (int r = 0; r < R; r++) t += fold[r][o];
           const int c = 8 * (o % T + T * i) + o / T;
-          if (c < p.cols) (which ? part_b : part_w)[c] = t;
+          if (c >= p.cols) continue;
+          if (p.part) (which ? part_b : part_w)[c] = t;
+          else store_elem(which ? p.dbias : p.dweight, p.weight_type, c, t);
         }
       }
     }
