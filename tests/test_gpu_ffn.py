@@ -521,6 +521,85 @@ def test_checkpoint_round_trip(gpu_api, rows, cols, typ, pad, skip):
     assert torch.equal(torch.nan_to_num(back.view.cpu(), nan=-1.25), torch.nan_to_num(O.checkpoint(x.view)[0].to(dt), nan=-1.25))
 
 
+# ---- offsets beyond 32 bits -------------------------------------------------------------------------------------------------
+
+def test_norm_and_checkpoint_beyond_32_bits(gpu_api):
+    """2.4e9 elements: the first and last rows, and some between"""
+    rows, cols = 290000, 8192
+    x = torch.empty(rows, cols, dtype=torch.bfloat16, device=DEV)
+    x.copy_(randn(1, 1000, cols).to(torch.bfloat16).repeat(rows // 1000, 1))
+    x[-1] = randn(2, cols) * 3
+    y, (codes, scales), back = torch.empty_like(x), ffn.checkpoint_buffers(rows, cols, DEV), torch.empty_like(x)
+    spec = dict(type=abi.CUDA_R_16BF, rows=rows, cols=cols)
+    ffn.NormForward(spec).run(x=x.data_ptr(), y=y.data_ptr(), stream=stream())
+    c = ffn.Checkpoint(spec)
+    c.store(x=x.data_ptr(), codes=codes.data_ptr(), scales=scales.data_ptr(), stream=stream())
+    c.load(codes=codes.data_ptr(), scales=scales.data_ptr(), x=back.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    for at in ([0, 1], [262143, 262144], [rows - 2, rows - 1]):
+        O.check(y[at], O.norm_forward(x[at], None, None, 1e-5)["y"], str(at))
+        value, code, scale = O.checkpoint(x[at])
+        assert torch.equal(codes[at].cpu(), code) and torch.equal(scales[at].cpu(), scale) and torch.equal(back[at].cpu(), value.to(torch.bfloat16))
+    mean, rstd = torch.zeros(rows, device=DEV), torch.ones(rows, device=DEV)
+    ffn.NormBackward(dict(spec, weights=False)).run(x=x.data_ptr(), dy=y.data_ptr(), mean=mean.data_ptr(), rstd=rstd.data_ptr(), dx=back.data_ptr(), stream=stream())
+    torch.cuda.synchronize()
+    for at in ([0, 1], [262143, 262144], [rows - 2, rows - 1]):
+        O.check(back[at], O.norm_backward(x[at], y[at], None, mean[at], rstd[at])["dx"], str(at))
+
+
+@pytest.mark.parametrize("which", ["x", "h"])
+def test_gated_forward_pitches_beyond_32_bits(gpu_api, which):
+    """rows 16 MiB apart: X (which leaves the 2 GiB windows), H and what is kept"""
+    t, d, f = 300, 128, 200
+    wide = 8 << 20
+    big = torch.empty(t * wide, dtype=torch.bfloat16, device=DEV)
+    far = big.view(t, wide)
+    x, w = randn(1, t, d).to(torch.bfloat16), randn(2, 2 * f, d, std=d ** -0.5).to(torch.bfloat16)
+    h = torch.empty(t, f, dtype=torch.bfloat16, device=DEV)
+    spec = dict(type=abi.CUDA_R_16BF, tokens=t, features=f, model=d, kept=ffn.KEPT_PLAIN)
+    if which == "x":
+        far[:, :d] = x
+        ffn.GatedForward(dict(spec, ldx=wide, kept=ffn.KEPT_NONE)).run(x=big.data_ptr(), w=w.data_ptr(), h=h.data_ptr(), stream=stream())
+        outs = {"h": h}
+    else:
+        ffn.GatedForward(dict(spec, ldh=wide, ldgate=wide, ldup=wide)).run(x=x.data_ptr(), w=w.data_ptr(), h=big.data_ptr(), gate=big.data_ptr() + 2000, up=big.data_ptr() + 4000,
+                                                                          stream=stream())
+        outs = {"h": far[:, :f], "g": far[:, 1000:1000 + f], "u": far[:, 2000:2000 + f]}
+    torch.cuda.synchronize()
+    ref = O.gated_forward("silu", x, w, None)
+    for k, v in outs.items():
+        O.check(v, ref[k], k)
+
+
+def test_gated_backward_beyond_32_bits(gpu_api):
+    """[dG dU] of 2.3e9 bytes: its last rows, the gradients that come from them, and a bias gradient over all rows"""
+    t, d, f = 42000, 64, 14336
+    bf = torch.bfloat16
+    rows = 500
+    dh, g, u = (randn(i, rows, f, std=0.7).to(bf).repeat(t // rows, 1) for i in range(3))
+    x, w = randn(4, t, d).to(bf), randn(5, 2 * f, d, std=0.1).to(bf)
+    dz, dx, dw, db = (torch.empty(s, dtype=bf, device=DEV) for s in ((t, 2 * f), (t, d), (2 * f, d), (2 * f,)))
+    call = ffn.GatedBackward(dict(type=abi.CUDA_R_16BF, tokens=t, features=f, model=d, bias=True, dz=True))
+    ws, _keep = scratch(call)
+    call.run(dh=dh.data_ptr(), gate=g.data_ptr(), up=u.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), dbias=db.data_ptr(), dz=dz.data_ptr(),
+             stream=stream(), **ws)
+    torch.cuda.synchronize()
+    for at in (slice(0, 3), slice(t - 3, t)):
+        ref = O.gated_backward("silu", dh[at], g[at], u[at], x[at], w)
+        O.check(dz[at], ref["dz"], "dz")
+        O.check(dx[at], ref["dx"], "dx")
+    # the rows repeat: their sums are those of one period times the periods, and dw that with X summed over the periods
+    one = O.gated_backward("silu", dh[:rows], g[:rows], u[:rows], x[:rows], w)
+    n = t // rows
+    value, bound = one["dbias"]
+    O.check(db, (n * value, n * bound + (t + 1) * O.E32 * n * (one["dz"][0].abs() + one["dz"][1]).sum(0)), "dbias")
+    xs = x.double().reshape(n, rows, d)
+    z, ez = one["dz"]
+    er = ez + O.UNIT[bf] * (z.abs() + ez) + O.TINY[bf]
+    mag = (z.abs() + er).t() @ xs.abs().sum(0)
+    O.check(dw, (z.t() @ xs.sum(0), er.t() @ xs.abs().sum(0) + (t + 1) * O.E32 * mag), "dw")
+
+
 # ---- streams and graphs -----------------------------------------------------------------------------------------------------
 
 def test_operators_in_a_graph_on_another_stream(gpu_api):
