@@ -120,6 +120,9 @@ __device__ __forceinline__ void ffn_with_act(uint32_t act, F &&f) {
 
 // ---- checkpoints ------------------------------------------------------------------------------------------------------------
 // Magnitude bits of a value as they count for a block's exponent: an integer order, and nothing that is not finite.
+// Almost every block is finite, and a wave finds that out from the plain maximum of the bits: only where one is not (a uniform
+// branch) are the values looked at one by one, and only there does the conversion have to turn infinities into NaN.
+constexpr uint32_t kCkptInf = 0x7f800000u;
 __device__ __forceinline__ uint32_t ckpt_mag(float v) {
   const uint32_t b = f2bits(v) & 0x7fffffffu;
   return b < 0x7f800000u ? b : 0u;
@@ -133,10 +136,11 @@ __device__ __forceinline__ uint32_t ckpt_scale_byte(uint32_t mag) {
 __device__ __forceinline__ float ckpt_scale(uint32_t byte) { return bits2f(byte << 23); }
 __device__ __forceinline__ float ckpt_inverse(uint32_t byte) { return bits2f((254u - byte) << 23); }  // (byte is 1 .. 247)
 
-// Four values to four codes; `inv` the inverse of the block's scale (a power of two: exact).  Infinities are turned into NaN
-// first (the instruction's own answer to them depends on a mode bit).
+// Four values to four codes; `inv` the inverse of the block's scale (a power of two: exact).  ODD: there may be values that are not
+// finite; infinities are turned into NaN first (the instruction's own answer to them depends on a mode bit).
+template <bool ODD>
 __device__ __forceinline__ uint32_t ckpt_encode4(float a, float b, float c, float d, float inv) {
-  auto fin = [&](float v) __attribute__((always_inline)) { return (v * inv) - (v - v); };  // (v - v: 0, or NaN for what is not finite)
+  auto fin = [&](float v) __attribute__((always_inline)) { return ODD ? (v * inv) - (v - v) : v * inv; };  // (v - v: 0, or NaN for what is not finite)
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(fin(a), fin(b), 0, false);
   w = __builtin_amdgcn_cvt_pk_fp8_f32(fin(c), fin(d), w, true);
   return (uint32_t)w;
@@ -158,13 +162,25 @@ __device__ __forceinline__ uint32_t ckpt_quad_max(uint32_t m) {
 // Eight values of a row (zeros past its end) to their place in a checkpoint.  Four neighbouring lanes hold a block, all four
 // of them active; a lane whose eight columns start at or past `cols32` (the row's blocks times 32) stores nothing.
 __device__ __forceinline__ void ckpt_store8(uint8_t *codes, uint8_t *scales, int col, int cols32, const float (&v)[8]) {
-  uint32_t m = ckpt_mag(v[0]);
+  uint32_t m = 0;
 #pragma unroll
-  for (int e = 1; e < 8; e++) m = max(m, ckpt_mag(v[e]));
-  const uint32_t byte = ckpt_scale_byte(ckpt_quad_max(m));
-  const float inv = ckpt_inverse(byte);
+  for (int e = 0; e < 8; e++) m = max(m, f2bits(v[e]) & 0x7fffffffu);
+  uint32_t byte;
+  ffn_u2 out;
+  if (__builtin_expect(__any(m >= kCkptInf), 0)) {
+    m = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) m = max(m, ckpt_mag(v[e]));
+    byte = ckpt_scale_byte(ckpt_quad_max(m));
+    const float inv = ckpt_inverse(byte);
+    out = ffn_u2{ckpt_encode4<true>(v[0], v[1], v[2], v[3], inv), ckpt_encode4<true>(v[4], v[5], v[6], v[7], inv)};
+  } else {
+    byte = ckpt_scale_byte(ckpt_quad_max(m));
+    const float inv = ckpt_inverse(byte);
+    out = ffn_u2{ckpt_encode4<false>(v[0], v[1], v[2], v[3], inv), ckpt_encode4<false>(v[4], v[5], v[6], v[7], inv)};
+  }
   if (col < cols32) {
-    *(ffn_u2 *)(codes + col) = ffn_u2{ckpt_encode4(v[0], v[1], v[2], v[3], inv), ckpt_encode4(v[4], v[5], v[6], v[7], inv)};
+    *(ffn_u2 *)(codes + col) = out;
     if ((col & 31) == 0) scales[col >> 5] = (uint8_t)byte;
   }
 }

@@ -53,7 +53,9 @@ __global__ __launch_bounds__(256) void gated_any_kernel(GatedParams p) {
       u[a][e] = acc[a + 2][e] + (p.bias ? E::dec(((const raw *)p.bias)[p.features + fe]) : 0.0f);
     }
   const int token = t0 + wave * 16 + r16;
-  gated_store<E, 2>(p, f0, token, token < p.tokens, g, u);
+  gated_with(p, [&](auto kept, auto act) __attribute__((always_inline)) {
+    gated_store<E, decltype(kept)::value, decltype(act)::value>(p, f0, token, token < p.tokens, g, u);
+  });
 }
 
 } // namespace zluda_amd

@@ -149,19 +149,21 @@ __global__ __launch_bounds__(64 * WP *WQ) void gated_tile_kernel(GatedTileParams
       bg[a][e] = p.bias ? E::dec(((const raw *)p.bias)[f]) : 0.0f;
       bu[a][e] = p.bias ? E::dec(((const raw *)p.bias)[p.features + f]) : 0.0f;
     }
+  gated_with(p, [&](auto kept, auto act) __attribute__((always_inline)) {
 #pragma unroll
-  for (int b = 0; b < TQ; b++) {
-    float g[TG][4], u[TG][4];
+    for (int b = 0; b < TQ; b++) {
+      float g[TG][4], u[TG][4];
 #pragma unroll
-    for (int a = 0; a < TG; a++)
+      for (int a = 0; a < TG; a++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        g[a][e] = acc[a][b][e] + bg[a][e];
-        u[a][e] = acc[a + TG][b][e] + bu[a][e];
-      }
-    const int token = t0 + wq * (16 * TQ) + 16 * b + r16;
-    gated_store<E, TG>(p, fw, token, token < p.tokens, g, u);
-  }
+        for (int e = 0; e < 4; e++) {
+          g[a][e] = acc[a][b][e] + bg[a][e];
+          u[a][e] = acc[a + TG][b][e] + bu[a][e];
+        }
+      const int token = t0 + wq * (16 * TQ) + 16 * b + r16;
+      gated_store<E, decltype(kept)::value, decltype(act)::value>(p, fw, token, token < p.tokens, g, u);
+    }
+  });
 }
 
 } // namespace zluda_amd

@@ -35,26 +35,28 @@ struct GatedMfmaParams : MfmaParams {
         }
     }
     __builtin_amdgcn_sched_barrier(0);
+    gated_with(gated, [&](auto kept, auto act) __attribute__((always_inline)) {
 #pragma unroll
-    for (int b = 0; b < TQ; b++) {
-      // (one column of tiles at a time, read explicitly: see w4_store_f16)
-      int raw[8][4];
+      for (int b = 0; b < TQ; b++) {
+        // (one column of tiles at a time, read explicitly: see w4_store_f16)
+        int raw[8][4];
 #pragma unroll
-      for (int a = 0; a < 8; a++)
+        for (int a = 0; a < 8; a++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) raw[a][e] = w4_acc_read(acc[a][b][e]);
-      float g[4][4], u[4][4];
+          for (int e = 0; e < 4; e++) raw[a][e] = w4_acc_read(acc[a][b][e]);
+        float g[4][4], u[4][4];
 #pragma unroll
-      for (int a = 0; a < 4; a++)
+        for (int a = 0; a < 4; a++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          g[a][e] = bits2f((uint32_t)raw[a][e]) + bg[a][e];
-          u[a][e] = bits2f((uint32_t)raw[a + 4][e]) + bu[a][e];
-        }
-      const int token = t0 + 16 * b + (lane & 15);
-      gated_store<E, 4>(gated, f0, token, token < gated.tokens, g, u);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+          for (int e = 0; e < 4; e++) {
+            g[a][e] = bits2f((uint32_t)raw[a][e]) + bg[a][e];
+            u[a][e] = bits2f((uint32_t)raw[a + 4][e]) + bu[a][e];
+          }
+        const int token = t0 + 16 * b + (lane & 15);
+        gated_store<E, decltype(kept)::value, decltype(act)::value>(gated, f0, token, token < gated.tokens, g, u);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    });
   }
 };
 
