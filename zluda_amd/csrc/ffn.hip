@@ -9,6 +9,7 @@
 #include "ffn_launch.hpp"
 #include "kernels/ffn_elementwise.hpp"
 #include "kernels/ffn_norm.hpp"
+#include "planner.hpp"
 
 using namespace zluda_amd;
 
@@ -189,7 +190,13 @@ uint32_t run_matmul(uint32_t type, uint32_t transa, uint32_t transb, uint64_t m,
   q.A = A; q.B = B; q.C = D; q.D = D;
   q.workspace = ws; q.workspace_size = ws_size;
   zluda_gemm_plan plan;
-  uint32_t st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_AUTO, -1, zluda_gemm_device_cu_count(), &plan);
+  // Tiles of 256 x 256 wherever they fill the chip twice; the planner's own choice, made from the time of a single stage, takes half-size ones
+  // for some of these (A:N B:T 2360 x 15440 x 6196, 610 tiles: 443 us on them, 557 on 128 x 128).
+  static_assert(kTrVariants[3].bp == 256 && kTrVariants[3].bq == 256, "the largest tile");
+  const uint32_t cu = zluda_gemm_device_cu_count();
+  uint32_t st = CUBLAS_STATUS_NOT_SUPPORTED;
+  if (((m + 255) / 256) * ((n + 255) / 256) >= 2ull * cu) st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_MFMA_TR16, 3, cu, &plan);
+  if (st != CUBLAS_STATUS_SUCCESS) st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_AUTO, -1, cu, &plan);
   if (st == CUBLAS_STATUS_SUCCESS) st = zluda_gemm_launch(&q, &plan, s);
   return st;
 }
