@@ -207,3 +207,20 @@ def test_the_oracle_s_checkpoint_against_the_formats():
     top = x.abs().double().reshape(40, 3, 32).amax(2)
     e = scales.double() - 127
     assert (top <= 448 * 2 ** e).all() and ((top > 448 * 2 ** (e - 1)) | (e == -126)).all()
+
+
+def test_workspace_of_a_product_in_parts():
+    """operands beyond 2 GiB: the 32-bit sum of dW comes on top, once; a pitch that no call takes is answered all the same"""
+    lib = ffn.load()
+
+    def bytes_of(**over):
+        n = C.c_size_t()
+        assert lib.zluda_ffn_gated_backward_workspace(C.byref(backward(**over)), C.byref(n)) == 0
+        return n.value
+
+    big = dict(tokens=40000, features=16384, model=2048, dz__data=64, dz__type=BF, dz__ld=32768, dx__ld=2048, dw__ld=2048, x__ld=2048, w__ld=2048, dh__ld=16384,
+               gate__ld=16384, up__ld=16384)
+    assert bytes_of(**big) - bytes_of(**dict(big, tokens=30000)) == 2 * 16384 * 2048 * 4
+    assert bytes_of(**dict(big, dw__data=None)) == bytes_of(**dict(big, dw__data=None, tokens=30000))
+    for ld in (0, -1, 1 << 62, -(1 << 63)):
+        bytes_of(x__ld=ld, dz__data=64, dz__ld=ld)

@@ -649,3 +649,44 @@ def test_operators_in_a_graph_on_another_stream(gpu_api):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, outs)), "replay %d" % r
         assert all(torch.isfinite(a.float()).all() for a in got)
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("which", ["x", "dz", "x_8bit"])
+def test_gated_in_parts(gpu_api, which, dt):
+    """rows so far apart that the matmuls take the tokens in two parts: X of the forward product, [dG dU] or X of the backward pass"""
+    t, d, f, wide = 2900, 136, 200, 400000
+    code = {torch.bfloat16: abi.CUDA_R_16BF, torch.float16: abi.CUDA_R_16F}[dt]
+    big = torch.empty(t * wide, dtype=dt, device=DEV)
+    far = big.view(t, wide)
+    x, w = randn(1, t, d).to(dt), randn(2, 2 * f, d, std=d ** -0.5).to(dt)
+    kept = ffn.KEPT_8BIT if which == "x_8bit" else ffn.KEPT_PLAIN
+    if which != "dz":
+        far[:, :d] = x
+        g, u = ([Ckpt(t, f), Ckpt(t, f)] if which == "x_8bit" else [Mat(t, f, dt), Mat(t, f, dt)])
+        h = torch.empty(t, f, dtype=dt, device=DEV)
+        args = dict(gate=g.codes.ptr, up=u.codes.ptr, gate_scales=g.scales.ptr, up_scales=u.scales.ptr) if which == "x_8bit" else dict(gate=g.ptr, up=u.ptr)
+        lds = dict(ldgate=g.codes.ld, ldup=u.codes.ld, ldgate_scales=g.scales.ld, ldup_scales=u.scales.ld) if which == "x_8bit" else dict(ldgate=g.ld, ldup=u.ld)
+        ffn.GatedForward(dict(type=code, tokens=t, features=f, model=d, ldx=wide, kept=kept, **lds)).run(x=big.data_ptr(), w=w.data_ptr(), h=h.data_ptr(), stream=stream(), **args)
+        torch.cuda.synchronize()
+        ref = O.gated_forward("silu", x, w, None)
+        O.check(h, ref["h"], "h")
+        if which == "x_8bit":
+            for m, name in ((g, "g"), (u, "u")):  # (half a step, as for the checkpoints of run_gated())
+                value, bound = ref[name]
+                top = torch.nn.functional.pad(value.abs() + bound, (0, -f % 32)).reshape(t, -1, 32).amax(2).repeat_interleave(32, 1)[:, :f]
+                assert ((m.values() - value).abs() <= (bound + (value.abs() + bound) * 2.0 ** -4 + top / 224 * 2.0 ** -10) * 1.001).all() and m.guards(), name
+            return
+        O.check(g.view, ref["g"], "g")
+        O.check(u.view, ref["u"], "u")
+    dh, gate, up = (randn(i, t, f, std=0.7).to(dt) for i in range(3, 6))
+    dx, dw, db = (torch.empty(s, dtype=dt, device=DEV) for s in ((t, d), (2 * f, d), (2 * f,)))
+    spec = dict(type=code, tokens=t, features=f, model=d, bias=True, dz=which == "dz", **({"lddz": wide} if which == "dz" else {"ldx": wide}))
+    call = ffn.GatedBackward(spec)
+    ws, _keep = scratch(call)
+    call.run(dh=dh.data_ptr(), gate=gate.data_ptr(), up=up.data_ptr(), x=big.data_ptr() if which == "x" else x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(),
+             dbias=db.data_ptr(), dz=big.data_ptr() if which == "dz" else None, stream=stream(), **ws)
+    torch.cuda.synchronize()
+    ref = O.gated_backward("silu", dh, gate, up, x, w)
+    for name, out in (("dx", dx), ("dw", dw), ("dbias", db)) + ((("dz", far[:, :2 * f]),) if which == "dz" else ()):
+        O.check(out, ref[name], name)
