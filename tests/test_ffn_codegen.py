@@ -9,7 +9,7 @@ import pytest
 import test_w4_codegen as w4
 
 CSRC = os.path.join(w4.ROOT, "zluda_amd", "csrc")
-FLAGS = {"ffn_small_bf16.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+FLAGS = {unit: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for unit in ("ffn_small_bf16.hip", "ffn_products.hip")}
 
 
 @pytest.mark.parametrize("unit", ["ffn_gated_bf16.hip", "ffn_gated_f16.hip"])
@@ -72,3 +72,25 @@ def test_tiles_hold_no_spills(tmp_path):
     found = re.findall(r"\.name:\s+(\S*gated_(?:tile|any)_kernel\S*).*?\.vgpr_spill_count:\s+(\d+)", text, re.S)
     assert len(found) == len(tiles()) + 1 and all(n == "0" for _, n in found), found
     assert "scratch_" not in text and "v_pk_fma_f32" not in text and "v_pk_mul_f32" not in text and "v_pk_add_f32" not in text
+
+
+def test_grad_products_stages(tmp_path):
+    """two stages of the loops of dX and dW: 32 MFMAs and 8 DMA instructions each, one barrier with a wait for everything; registers and LDS of two
+    workgroups a CU"""
+    import subprocess
+    out = str(tmp_path / "k.s")
+    cmd = [w4.HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", *FLAGS["ffn_products.hip"],
+           "--cuda-device-only", "-S", os.path.join(CSRC, "ffn_products.hip"), "-o", out]
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    assert res.returncode == 0, res.stdout[-2000:]
+    text = open(out).read()
+    assert "scratch_" not in text and "v_accvgpr_" not in text and "v_pk_" not in re.sub(r"v_pk_(mov|lshl|or|and)", "", text)
+    meta = re.findall(r"\.group_segment_fixed_size: (\d+).*?\.name:\s+\S*grad_products_kernel\S*.*?\.vgpr_count:\s+(\d+)", text, re.S)
+    assert len(meta) == 2 and all(int(lds) * 2 <= 160 * 1024 and int(regs) <= 256 for lds, regs in meta), meta
+    for m in re.finditer(r"^(_ZN9zluda_amd20grad_products_kernel\w+):\s*;.*?\n(.*?)^\.Lfunc_end", text, re.S | re.M):
+        blocks = re.split(r"^\.LBB\d+_\d+:", m.group(2), flags=re.M)
+        loops = [b for b in blocks if b.count("v_mfma") == 64]
+        assert len(loops) == 2, m.group(1)
+        for b in loops:
+            assert len(re.findall(r"buffer_load_dwordx4.* lds", b)) == 16 and b.count("s_barrier") == 2 and b.count("s_waitcnt vmcnt(0)") == 2
+        assert sorted((b.count("ds_read_b64_tr_b16"), b.count("ds_read_b128")) for b in loops) == [(32, 16), (64, 0)]

@@ -246,6 +246,19 @@ def test_gated_backward_sizes(gpu_api, typ, t, d, f):
             check_gated_backward(outs, ref, what)
 
 
+# sizes of the launch that makes dx and dw together (16-byte pieces): edges of its tiles and stages, and K of dx in one share and in many
+@pytest.mark.parametrize("t,d,f", [(1, 8, 4), (2, 136, 60), (63, 128, 64), (64, 128, 68), (65, 120, 132), (127, 256, 200), (128, 264, 64), (129, 136, 300), (300, 520, 256),
+                                   (1000, 136, 2052), (640, 1032, 128), (1, 1024, 4096)])
+@pytest.mark.parametrize("pad", [0, 8, 72])
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+def test_gated_backward_products_together(gpu_api, typ, pad, t, d, f):
+    for kept in (ffn.KEPT_PLAIN, ffn.KEPT_8BIT):
+        what = "gated backward %s %d x %d x %d pad %d kept %d" % (typ, t, d, f, pad, kept)
+        print(what, flush=True)
+        outs, ref, _ = run_gated_backward(typ, "gelu", t, d, f, kept, pad, pad, seed=t)
+        check_gated_backward(outs, ref, what)
+
+
 @pytest.mark.parametrize("pad,skip", [(1, 0), (0, 3), (8, 8)])
 @pytest.mark.parametrize("want", [("dx",), ("dw",), ("dx", "dw"), ("dbias",), ("h", "dz"), ("dw", "dbias")])
 def test_gated_backward_pitches_and_choices(gpu_api, want, pad, skip):

@@ -9,6 +9,7 @@
 #include "ffn_launch.hpp"
 #include "kernels/ffn_elementwise.hpp"
 #include "kernels/ffn_norm.hpp"
+#include "kernels/store_window.hpp"
 #include "planner.hpp"
 
 using namespace zluda_amd;
@@ -82,13 +83,44 @@ uint64_t rows_in_window(uint64_t rows, int64_t ld) {
   const int64_t most = ld < 1 ? 0 : (0x3fffffffll / ld - 256) & ~255ll;  // (a workspace is asked for before pitches are checked)
   return most > 0 && rows > (uint64_t)most ? (uint64_t)most : rows;
 }
+bool in_window(uint64_t rows, int64_t ld) { return (int64_t)(rows + 256) <= 0x3fffffffll / ld; }
+
+// dX and dW in one launch of 128 x 128 tiles (kernels/ffn_grad_products.hpp), or one after the other on the framework's matmul kernels?  Together, us
+// of whole backward passes and in brackets one after the other: 64 tokens, 4096 x 14336 124 (158), 300, 2048 x 5632 54 (67), 700, 4096 x 14336
+// 389 (438), 1100 594 (663), 1001, 1024 x 2816 48 (53), 1500, 2048 x 8192 230 (262), 5000, 1024 x 8192 388 (465), 3000, 4096 x 2816 284 (286).
+// One after the other
+//  * where both fill the chip by themselves, dW twice with tiles of 256 x 256, which compute faster (2000, 4096 x 11008 758 and 709; 8192, 2048 x
+//    8192 1152 and 925);
+//  * where a tile of dW alone takes more than twice the time all tiles take the chip: its K is not shared out here (8192, 1024 x 512 105 and 60;
+//    3000, 512 x 512 38 and 33; with as much as twice 4096, 1024 x 1024 61 and 64, 8192, 512 x 2048 148 and 131).
+// The shares of dX's K are no longer than that time either, or than a tile of dW (1001, 1024 x 2816 in 1, 2, 3, 4 shares 70, 48, 45, 48; 64, 1024 x 2816
+// in 3, 8, 12 31, 21, 21; 2000, 1024 x 1024, a share as long as a tile of dW, in 1 and 2 32 and 41).
+struct GradTogether {
+  uint32_t splits, split_stages;  // shares of dX's K; 0: one after the other
+  uint64_t part;                  // bytes of their sums
+};
+GradTogether grad_together(const zluda_ffn_gated_grad *p) {
+  GradTogether g{0, 0, 0};
+  if (!p->dx.data || !p->dw.data || !p->tokens || p->model % 8 || p->features % 4) return g;
+  auto tiles = [](uint64_t a, uint64_t b, uint64_t side) { return ((a + side - 1) / side) * ((b + side - 1) / side); };
+  const uint64_t f2 = 2 * p->features, slots = 2 * (uint64_t)cus(), n_dx = tiles(p->model, p->tokens, kGradTile), n_dw = tiles(p->model, f2, kGradTile);
+  const uint64_t k_dx = (f2 + kGradStage - 1) / kGradStage, k_dw = (p->tokens + kGradStage - 1) / kGradStage;
+  const uint64_t all = (n_dx * k_dx + n_dw * k_dw + slots - 1) / slots;  // stages of a workgroup if they were shared out evenly
+  if ((n_dx >= slots && tiles(p->model, f2, 256) >= slots) || k_dw > 2 * all) return g;
+  const uint64_t each = std::max(all, k_dw), want = std::min<uint64_t>(16, (k_dx + each - 1) / each);
+  g.split_stages = (uint32_t)((k_dx + want - 1) / want);
+  g.splits = (uint32_t)((k_dx + g.split_stages - 1) / g.split_stages);
+  g.part = g.splits > 1 ? g.splits * n_dx * kGradTile * kGradTile * 4 : 0;
+  return g;
+}
 
 // where the parts of the backward pass's workspace lie
 struct GradPlan {
   uint64_t dz, x, sums, gemm, acc, total;  // offsets
   uint64_t dx_rows, dw_rows;               // tokens of a matmul
   int64_t lddz;
-  uint32_t shares;                    // partial rows of dbias
+  uint32_t shares;                         // partial rows of dbias
+  GradTogether together;
 };
 
 // Workgroups of gated_grad_kernel along the rows.  Without sums a row of its own for every thread (8192 x 8192: 112 us, 130 with eight
@@ -110,6 +142,7 @@ GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
   uint64_t at = 0;
   g.lddz = p->dz.data ? p->dz.ld : aligned_pitch(2 * p->features);
   g.shares = grad_shares(p->tokens, p->features, p->dbias != nullptr);
+  g.together = grad_together(p);
   g.dz = at;
   if (!p->dz.data) at += aligned256(p->tokens * (uint64_t)g.lddz * 2);
   g.x = at;
@@ -117,7 +150,7 @@ GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
   g.sums = at;
   if (p->dbias) at += aligned256((uint64_t)g.shares * 2 * p->features * 4);
   g.gemm = at;
-  if (p->dx.data || p->dw.data) at += kGemmWorkspace;
+  if (p->dx.data || p->dw.data) at += std::max<uint64_t>(kGemmWorkspace, g.together.part);
   // dW over several parts is summed in 32 bits and rounded once
   g.acc = at;
   g.dx_rows = rows_in_window(p->tokens, g.lddz);
@@ -219,6 +252,33 @@ uint32_t run_matmul(uint32_t type, uint32_t transa, uint32_t transb, uint64_t m,
 uint32_t zero_rows(void *p, uint64_t rows, uint64_t row_bytes, int64_t pitch_bytes, hipStream_t s) {
   const ZeroParams z{p, (int64_t)rows, (int64_t)row_bytes, pitch_bytes};
   return launch_kernel(zero_rows_kernel, dim3((uint32_t)std::min<uint64_t>(2048, (rows * row_bytes / 2 + 255) / 256)), dim3(256), s, z);
+}
+
+uint32_t round_rows(uint32_t type, const RoundParams &r, hipStream_t s) {
+  const dim3 grid((uint32_t)((r.cols + 511) / 512), (uint32_t)std::min<int64_t>((r.rows + 3) / 4, kGridY));
+  return type == CUDA_R_16BF ? launch_kernel(round_rows_kernel<ElemBF16>, grid, dim3(256), s, r) : launch_kernel(round_rows_kernel<ElemF16>, grid, dim3(256), s, r);
+}
+
+// 16-byte pieces of all operands and results, through windows of 2 GiB
+bool grad_together_operands(const zluda_ffn_gated_grad *p, const zluda_ffn_matrix &x, const GradPlan &plan, const void *dz) {
+  return !((p->w.ld | x.ld | plan.lddz | p->dx.ld | p->dw.ld) & 7) && p->dx.ld < kNarrowPitch && p->dw.ld < kNarrowPitch &&
+         !(((uintptr_t)p->w.data | (uintptr_t)x.data | (uintptr_t)dz | (uintptr_t)p->dx.data | (uintptr_t)p->dw.data) & 15) && in_window(p->tokens, x.ld) &&
+         in_window(p->tokens, plan.lddz) && in_window(2 * p->features, p->w.ld);
+}
+
+// the two products in one launch, and the sums of dX's shares
+uint32_t run_together(uint32_t type, const zluda_ffn_gated_grad *p, const zluda_ffn_matrix &x, const GradPlan &plan, const void *dz, float *part, hipStream_t s) {
+  const GradTogether &t = plan.together;
+  const int model = (int)p->model, tokens = (int)p->tokens, f2 = (int)(2 * p->features);
+  auto tiles = [](int n) { return (n + kGradTile - 1) / kGradTile; };
+  GradProductsParams m;
+  m.dx = {p->w.data, dz, p->dx.data, part, p->dx.ld, (int32_t)p->w.ld, (int32_t)plan.lddz, model, tokens, f2, tiles(model), tiles(tokens), (int32_t)t.splits, (int32_t)t.split_stages};
+  m.dw = {x.data, dz, p->dw.data, nullptr, p->dw.ld, (int32_t)x.ld, (int32_t)plan.lddz, model, f2, tokens, tiles(model), tiles(f2), 1, (tokens + kGradStage - 1) / kGradStage};
+  m.dx_groups = (uint32_t)(m.dx.tiles_p * m.dx.tiles_q) * t.splits;
+  FFN_CHECK(launch_grad_products(type, m, s));
+  if (t.splits == 1) return CUBLAS_STATUS_SUCCESS;
+  const int64_t pitch = (int64_t)m.dx.tiles_p * kGradTile;
+  return round_rows(type, {part, p->dx.data, tokens, pitch, p->dx.ld, pitch * m.dx.tiles_q * kGradTile, model, (int32_t)t.splits}, s);
 }
 
 // ---- layer norm ---------------------------------------------------------------------------------------------------------------
@@ -373,6 +433,7 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
   const uint64_t f2 = 2 * p->features;
   // row-major matrices are column-major ones transposed: dx^T = W^T dz^T, dw^T = x^T dz
   auto rows_of = [](const void *m, int64_t ld, uint64_t row) { return (char *)m + row * ld * 2; };
+  if (plan.together.splits && grad_together_operands(p, x, plan, g.dz)) return run_together(type, p, x, plan, g.dz, (float *)gemm_ws, s);
   if (p->dx.data)
     for (uint64_t t = 0; t < p->tokens; t += plan.dx_rows)
       FFN_CHECK(run_matmul(type, CUBLAS_OP_N, CUBLAS_OP_N, p->model, std::min(plan.dx_rows, p->tokens - t), f2, p->w.data, p->w.ld, rows_of(g.dz, plan.lddz, t), plan.lddz,
@@ -384,11 +445,7 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
     for (uint64_t t = 0; t < p->tokens; t += plan.dw_rows)
       FFN_CHECK(run_matmul(type, CUBLAS_OP_N, CUBLAS_OP_T, p->model, f2, std::min(plan.dw_rows, p->tokens - t), rows_of(x.data, x.ld, t), x.ld, rows_of(g.dz, plan.lddz, t),
                            plan.lddz, parts ? CUDA_R_32F : type, t ? 1.0f : 0.0f, sum, ld_sum, gemm_ws, kGemmWorkspace, s));
-    if (parts) {
-      const RoundParams r{(const float *)sum, p->dw.data, (int64_t)f2, ld_sum, p->dw.ld, (int32_t)p->model};
-      const dim3 grid((uint32_t)((p->model + 511) / 512), (uint32_t)std::min<uint64_t>((f2 + 3) / 4, kGridY));
-      FFN_CHECK(type == CUDA_R_16BF ? launch_kernel(round_rows_kernel<ElemBF16>, grid, dim3(256), s, r) : launch_kernel(round_rows_kernel<ElemF16>, grid, dim3(256), s, r));
-    }
+    if (parts) FFN_CHECK(round_rows(type, {(const float *)sum, p->dw.data, (int64_t)f2, ld_sum, p->dw.ld, 0, (int32_t)p->model, 1}, s));
   }
   return CUBLAS_STATUS_SUCCESS;
 }

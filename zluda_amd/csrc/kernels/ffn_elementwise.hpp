@@ -46,20 +46,24 @@ __global__ __launch_bounds__(256) void checkpoint_load_kernel(CheckpointParams p
 struct RoundParams {
   const float *x;
   void *y;
-  int64_t rows, ldx, ldy;
-  int32_t cols;
+  int64_t rows, ldx, ldy, plane;
+  int32_t cols, shares;
 };
 
-// Sums held in 32 bits to their type (rows of x on 16 bytes and padded to whole pieces)
+// Sums held in 32 bits to their type: the shares of x, `plane` elements apart, added in order (rows of x on 16 bytes and padded to whole pieces)
 template <class E>
 __global__ __launch_bounds__(256) void round_rows_kernel(RoundParams p) {
   const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63));
   if (col >= p.cols) return;
   for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < p.rows; row += gridDim.y * 4) {
-    const typename ElemF32::Raw8 r = load8<ElemF32>(p.x + row * p.ldx + col, 8);
-    float v[8];
+    const float *x = p.x + row * p.ldx + col;
+    float v[8] = {};
+#pragma unroll 4
+    for (int z = 0; z < p.shares; z++, x += p.plane) {
+      const typename ElemF32::Raw8 r = load8<ElemF32>(x, 8);
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = ElemF32::get(r, e);
+      for (int e = 0; e < 8; e++) v[e] += ElemF32::get(r, e);
+    }
     store8<E>((typename E::raw *)p.y + row * p.ldy + col, v, p.cols - col);
   }
 }
