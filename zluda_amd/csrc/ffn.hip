@@ -86,19 +86,33 @@ uint64_t rows_in_window(uint64_t rows, int64_t ld) {
 bool in_window(uint64_t rows, int64_t ld) { return (int64_t)(rows + 256) <= 0x3fffffffll / ld; }
 
 // dX and dW in one launch of 128 x 128 tiles (kernels/ffn_grad_products.hpp), or one after the other on the framework's matmul kernels?  Together, us
-// of whole backward passes and in brackets one after the other: 64 tokens, 4096 x 14336 124 (158), 300, 2048 x 5632 54 (67), 700, 4096 x 14336
-// 389 (438), 1100 594 (663), 1001, 1024 x 2816 48 (53), 1500, 2048 x 8192 230 (262), 5000, 1024 x 8192 388 (465), 3000, 4096 x 2816 284 (286).
+// of whole backward passes and in brackets one after the other: 64 tokens, 4096 x 14336 118 (167), 300, 2048 x 5632 59 (70), 700, 4096 x 14336
+// 399 (451), 1100 594 (663), 1001, 1024 x 2816 46 (55), 1500, 2048 x 8192 238 (270), 5000, 1024 x 8192 388 (465), 3000, 4096 x 2816 284 (286).
 // One after the other
 //  * where both fill the chip by themselves, dW twice with tiles of 256 x 256, which compute faster (2000, 4096 x 11008 758 and 709; 8192, 2048 x
 //    8192 1152 and 925);
 //  * where a tile of dW alone takes more than twice the time all tiles take the chip: its K is not shared out here (8192, 1024 x 512 105 and 60;
 //    3000, 512 x 512 38 and 33; with as much as twice 4096, 1024 x 1024 61 and 64, 8192, 512 x 2048 148 and 131).
-// The shares of dX's K are no longer than that time either, or than a tile of dW (1001, 1024 x 2816 in 1, 2, 3, 4 shares 70, 48, 45, 48; 64, 1024 x 2816
-// in 3, 8, 12 31, 21, 21; 2000, 1024 x 1024, a share as long as a tile of dW, in 1 and 2 32 and 41).
 struct GradTogether {
   uint32_t splits, split_stages;  // shares of dX's K; 0: one after the other
   uint64_t part;                  // bytes of their sums
 };
+// Stages until the launch is done, of `slots` workgroups at a time that take dX's n_dx * s shares, then the tiles of dW: half way between an even load
+// and one workgroup after the other at an even pace (one without a neighbour is faster, but not by as much).  A tile's start and end are as
+// long as three stages; a stage of a share takes `pace` quarters more than one at an even load, as it waits for W; the shares' sums are written and
+// read again, in a launch of their own.  Measured, us, shares of dX and times: 1001, 1024 x 2816 1: 71, 2: 49, 3: 46, 4: 49, 8: 49; 300, 2048 x 5632 3: 60,
+// 5: 56, 8: 57; 700, 4096 x 14336 1: 459, 2: 393, 3: 415; 2000, 1024 x 1024 1: 32, 2: 41; W from memory: 150, 4096 x 14336 3: 195, 5: 169, 8: 168, 12: 176;
+// 64, 4096 x 14336 3: 181, 8: 118, 12: 131; 100, 5120 x 13824 3: 198, 5: 164, 8: 168.
+double grad_together_stages(uint64_t slots, uint64_t n_dx, uint64_t k_dx, uint64_t n_dw, uint64_t k_dw, uint64_t s, uint64_t pace) {
+  const uint64_t l1 = (k_dx + s - 1) / s + 3, l2 = k_dw + 3, n1 = n_dx * s, even = (n1 * l1 + n_dw * l2) / slots, rounds = n1 / slots, rest = n1 % slots;
+  uint64_t low = std::max(even, rounds * l1 + (rest ? l1 + l1 * pace / 4 : 0)), high = low + l1 + (n_dw / slots + 2) * l2;  // (dW's tiles fit behind `high`)
+  while (low < high) {
+    const uint64_t end = (low + high) / 2, early = end > rounds * l1 ? (end - rounds * l1) / l2 : 0, late = end > (rounds + 1) * l1 ? (end - (rounds + 1) * l1) / l2 : 0;
+    if ((slots - rest) * early + rest * late >= n_dw) high = end;
+    else low = end + 1;
+  }
+  return 0.5 * (double)(even + low) + (s > 1 ? 5.0 + 0.04 * (double)n1 : 0.0);
+}
 GradTogether grad_together(const zluda_ffn_gated_grad *p) {
   GradTogether g{0, 0, 0};
   if (!p->dx.data || !p->dw.data || !p->tokens || p->model % 8 || p->features % 4) return g;
@@ -107,7 +121,16 @@ GradTogether grad_together(const zluda_ffn_gated_grad *p) {
   const uint64_t k_dx = (f2 + kGradStage - 1) / kGradStage, k_dw = (p->tokens + kGradStage - 1) / kGradStage;
   const uint64_t all = (n_dx * k_dx + n_dw * k_dw + slots - 1) / slots;  // stages of a workgroup if they were shared out evenly
   if ((n_dx >= slots && tiles(p->model, f2, 256) >= slots) || k_dw > 2 * all) return g;
-  const uint64_t each = std::max(all, k_dw), want = std::min<uint64_t>(16, (k_dx + each - 1) / each);
+  const uint64_t pace = 8 * p->features * p->model > 256ull << 20 ? 2 : 1;  // (W and dW are more than the memory-side cache)
+  uint64_t want = 1;
+  double best = 0.0;
+  for (uint64_t n = 1; n <= std::min<uint64_t>(16, k_dx); n++) {
+    const double stages = grad_together_stages(slots, n_dx, k_dx, n_dw, k_dw, n, pace);
+    if (n == 1 || stages < best) {
+      want = n;
+      best = stages;
+    }
+  }
   g.split_stages = (uint32_t)((k_dx + want - 1) / want);
   g.splits = (uint32_t)((k_dx + g.split_stages - 1) / g.split_stages);
   g.part = g.splits > 1 ? g.splits * n_dx * kGradTile * kGradTile * 4 : 0;
@@ -266,15 +289,16 @@ bool grad_together_operands(const zluda_ffn_gated_grad *p, const zluda_ffn_matri
          in_window(p->tokens, plan.lddz) && in_window(2 * p->features, p->w.ld);
 }
 
-// the two products in one launch, and the sums of dX's shares
-uint32_t run_together(uint32_t type, const zluda_ffn_gated_grad *p, const zluda_ffn_matrix &x, const GradPlan &plan, const void *dz, float *part, hipStream_t s) {
+// the two products and the bias gradient in one launch, then the sums of dX's shares
+uint32_t run_together(uint32_t type, const zluda_ffn_gated_grad *p, const zluda_ffn_matrix &x, const GradPlan &plan, const GatedGradParams &g, float *part, hipStream_t s) {
   const GradTogether &t = plan.together;
   const int model = (int)p->model, tokens = (int)p->tokens, f2 = (int)(2 * p->features);
   auto tiles = [](int n) { return (n + kGradTile - 1) / kGradTile; };
   GradProductsParams m;
-  m.dx = {p->w.data, dz, p->dx.data, part, p->dx.ld, (int32_t)p->w.ld, (int32_t)plan.lddz, model, tokens, f2, tiles(model), tiles(tokens), (int32_t)t.splits, (int32_t)t.split_stages};
-  m.dw = {x.data, dz, p->dw.data, nullptr, p->dw.ld, (int32_t)x.ld, (int32_t)plan.lddz, model, f2, tokens, tiles(model), tiles(f2), 1, (tokens + kGradStage - 1) / kGradStage};
+  m.dx = {p->w.data, g.dz, p->dx.data, part, p->dx.ld, (int32_t)p->w.ld, (int32_t)plan.lddz, model, tokens, f2, tiles(model), tiles(tokens), (int32_t)t.splits, (int32_t)t.split_stages};
+  m.dw = {x.data, g.dz, p->dw.data, nullptr, p->dw.ld, (int32_t)x.ld, (int32_t)plan.lddz, model, f2, tokens, tiles(model), tiles(f2), 1, (tokens + kGradStage - 1) / kGradStage};
   m.dx_groups = (uint32_t)(m.dx.tiles_p * m.dx.tiles_q) * t.splits;
+  m.sums = g.part; m.dbias = p->dbias; m.shares = (int32_t)plan.shares;
   FFN_CHECK(launch_grad_products(type, m, s));
   if (t.splits == 1) return CUBLAS_STATUS_SUCCESS;
   const int64_t pitch = (int64_t)m.dx.tiles_p * kGradTile;
@@ -425,15 +449,15 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
   }
   FFN_CHECK(type == CUDA_R_16BF ? (ck ? launch_gated_grad<ElemBF16, true>(g, plan.shares, s) : launch_gated_grad<ElemBF16, false>(g, plan.shares, s))
                                 : (ck ? launch_gated_grad<ElemF16, true>(g, plan.shares, s) : launch_gated_grad<ElemF16, false>(g, plan.shares, s)));
+  void *gemm_ws = ws + plan.gemm;
+  if (plan.together.splits && grad_together_operands(p, x, plan, g.dz)) return run_together(type, p, x, plan, g, (float *)gemm_ws, s);
   if (p->dbias) {
     NormFinishParams f{g.part, p->dbias, nullptr, (int32_t)plan.shares, (int32_t)(2 * p->features), type};
     FFN_CHECK(launch_kernel(norm_finish_kernel<16, 64>, dim3((uint32_t)((2 * p->features + 15) / 16), 1), dim3(1024), s, f));
   }
-  void *gemm_ws = ws + plan.gemm;
   const uint64_t f2 = 2 * p->features;
   // row-major matrices are column-major ones transposed: dx^T = W^T dz^T, dw^T = x^T dz
   auto rows_of = [](const void *m, int64_t ld, uint64_t row) { return (char *)m + row * ld * 2; };
-  if (plan.together.splits && grad_together_operands(p, x, plan, g.dz)) return run_together(type, p, x, plan, g.dz, (float *)gemm_ws, s);
   if (p->dx.data)
     for (uint64_t t = 0; t < p->tokens; t += plan.dx_rows)
       FFN_CHECK(run_matmul(type, CUBLAS_OP_N, CUBLAS_OP_N, p->model, std::min(plan.dx_rows, p->tokens - t), f2, p->w.data, p->w.ld, rows_of(g.dz, plan.lddz, t), plan.lddz,

@@ -37,6 +37,10 @@ struct GradProduct {
 struct GradProductsParams {
   GradProduct dx, dw;
   uint32_t dx_groups;  // the first workgroups' product is dX, whose shares of K take longest
+  // the bias gradient: the sum of `shares` rows of `sums`, at the end of the grid; NULL: none
+  const float *sums;
+  void *dbias;
+  int32_t shares;
 };
 constexpr int kGradTile = 128, kGradStage = 64;
 uint32_t launch_grad_products(uint32_t type, const GradProductsParams &p, hipStream_t s);

@@ -1,7 +1,7 @@
 // The two matrix products behind the gated layer's backward pass in one launch, in tiles of 128 x 128:
 //   dX^T [model][token] = sum over 2 features of W[f][model] dZ[token][f],   dW^T [model][f] = sum over tokens of X[token][model] dZ[token][f].
 // Both have 2 x tokens x 2 features x model operations and neither needs the other.  Launched one after the other each leaves a part of the chip idle
-// while its last tiles run, and dX, with few tiles of a long K, all the time; together they fill each other's gaps.
+// while its last tiles run, and dX, with few tiles of a long K, all the time; together they fill each other's gaps.  (The last sums of the bias gradient ride along.)
 //
 // One operand (P: W or X) lies along its row index `model`, the other (Q: dZ) along K for dX and along its row index for dW.  Stages of 64 K
 // elements travel straight into two slots of LDS; what lies along its row index is transposed by the LDS reads (ds_read_b64_tr_b16).  The layouts
@@ -9,8 +9,8 @@
 // fragments of the one arrive while the products of the other run.  The barrier lies between them: behind it stage kt + 1 has landed and every
 // wave has the fragments of stage kt, whose slot takes stage kt + 2.  Two workgroups share a CU, and one computes while the other waits.
 //
-// K rows past the end, whole stages of them among these, are requested out of the buffer windows' range and become zeros; every wait is for
-// everything in flight, so that it does not matter in which order such requests retire.
+// K rows past the end are requested out of the buffer windows' range and become zeros; every wait is for everything in flight, so that it does not
+// matter in which order such requests retire.  (Whole stages past the end requested like that cost 7 % at three stages, 150 tokens.)
 #pragma once
 #include "../ffn_launch.hpp"
 #include "ffn_gated_any.hpp"
@@ -90,36 +90,46 @@ __device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t
     for (int b = 0; b < TQ; b++) acc[a][b] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 
   static_for<8>([&](auto i_c) { issue(i_c, 0, 0); });
-  static_for<8>([&](auto i_c) { issue(i_c, 1, 1); });
+  if (stages > 1) static_for<8>([&](auto i_c) { issue(i_c, 1, 1); });
   wait_vmcnt_barrier<0>();
   using C0 = std::integral_constant<int, 0>;
   using C1 = std::integral_constant<int, 1>;
   static_for<TP + TQ>([&](auto i_c) { read(i_c, C0{}, 0); });
-  // the products of half `h`, behind them the fragments of the other half from `slot` and, behind the second, the requests for stage `kt`
-  auto half = [&](auto h_c, int slot, int kt) __attribute__((always_inline)) {
+  // the products of half `h`, behind them the fragments of the other half from `slot` and, where `more`, the requests for stage `kt`
+  auto half = [&](auto h_c, int slot, auto more_c, int kt) __attribute__((always_inline)) {
     constexpr int h = decltype(h_c)::value;
     static_for<TP * TQ>([&](auto x_c) {
       constexpr int x = decltype(x_c)::value, a = x / TQ, b = x % TQ;
       ffn_mfma<E>(fr[h][a], fr[h][TP + b], acc[a][b]);
       if constexpr (x < TP + TQ) read(x_c, std::integral_constant<int, 1 - h>{}, slot);
-      if constexpr (h == 1 && x < 8) issue(x_c, kt, 1 - slot);
+      if constexpr (decltype(more_c)::value != 0 && x < 8) issue(x_c, kt, 1 - slot);
       __builtin_amdgcn_sched_barrier(0);
     });
   };
-  auto do_stage = [&](auto slot_c, int kt) __attribute__((always_inline)) {
+  // `inside`: stage kt + 2 exists
+  auto do_stage = [&](auto slot_c, auto inside_c, int kt) __attribute__((always_inline)) {
     constexpr int slot = decltype(slot_c)::value;
-    half(C0{}, slot, 0);
+    half(C0{}, slot, C0{}, 0);
     wait_vmcnt_barrier<0>();
     __builtin_amdgcn_sched_barrier(0);
-    half(C1{}, 1 - slot, kt + 2);
+    if constexpr (decltype(inside_c)::value == 0) {
+      if (kt + 2 < stages) static_for<8>([&](auto i_c) { issue(i_c, kt + 2, slot); });
+    }
+    half(C1{}, 1 - slot, inside_c, kt + 2);
   };
   int kt = 0;
-  for (; kt + 2 <= stages; kt += 2) {
-    do_stage(C0{}, kt);
-    do_stage(C1{}, kt + 1);
+  for (; kt + 4 <= stages; kt += 2) {
+    do_stage(C0{}, C1{}, kt);
+    do_stage(C1{}, C1{}, kt + 1);
   }
-  if (kt < stages) do_stage(C0{}, kt);
-  __builtin_amdgcn_s_waitcnt(0);  // (nothing is on its way to LDS when the wave ends)
+  // one to three are left (what is read behind the last one is not used)
+  if (kt < stages) {
+    do_stage(C0{}, C0{}, kt);
+    if (kt + 1 < stages) {
+      do_stage(C1{}, C0{}, kt + 1);
+      if (kt + 2 < stages) do_stage(C0{}, C0{}, kt + 2);
+    }
+  }
 
   // ---- D: a lane has P rows 4 g4 .. + 3 of a tile, column r16 ----------------------------------------------------------------------------
   const int pc = p0 + wp * TP * 16, qc = q0 + wq * TQ * 16;
@@ -153,11 +163,28 @@ __device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t
     }
 }
 
+// 64 columns of the bias gradient: every fourth row to a wave, then the four sums in order.  (A launch of its own for it takes 4 us.)
+template <class E>
+__device__ __forceinline__ void grad_bias_sums(const GradProductsParams &p, int strip, float *lds) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = strip * 64 + lane, cols = p.dw.nq;
+  float sum = 0.0f;
+  if (col < cols) {
+    const float *from = p.sums + col;
+#pragma unroll 8
+    for (int z = wave; z < p.shares; z += 4) sum += from[(int64_t)z * cols];
+  }
+  lds[threadIdx.x] = sum;
+  __syncthreads();
+  if (wave == 0 && col < cols) ((typename E::raw *)p.dbias)[col] = E::enc(((lds[lane] + lds[lane + 64]) + lds[lane + 128]) + lds[lane + 192]);
+}
+
 template <class E>
 __global__ __launch_bounds__(256, 2) void grad_products_kernel(GradProductsParams prm) {
   __shared__ v4i lds[2 * kGradSlot];
+  const uint32_t dw_groups = (uint32_t)(prm.dw.tiles_p * prm.dw.tiles_q), id = blockIdx.x - prm.dx_groups;
   if (blockIdx.x < prm.dx_groups) grad_product_tile<E, false>(prm.dx, blockIdx.x, lds);
-  else grad_product_tile<E, true>(prm.dw, blockIdx.x - prm.dx_groups, lds);
+  else if (id < dw_groups) grad_product_tile<E, true>(prm.dw, id, lds);
+  else grad_bias_sums<E>(prm, (int)(id - dw_groups), (float *)lds);
 }
 
 } // namespace zluda_amd
