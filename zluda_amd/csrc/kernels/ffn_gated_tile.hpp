@@ -1,8 +1,8 @@
 // Gated feed-forward products in tiles of BF features and BT tokens, one a workgroup, from a single token on up to where the
 // persistent kernel has enough tiles.
 //
-// Few tokens are bound by the read of W: one token, 4096 x 14336, takes 42.7 us (235 MB at 5.5 TB/s; a large copy moves 5.2), 32
-// tokens 43.0, 64 tokens (64 x 64 tiles) 46.2.  More are bound by the matrix cores and LDS: 256 tokens (128 x 128) 74 us, 810 TFLOP/s.
+// Few tokens are bound by the read of W: one token, 4096 x 14336, takes 41.0 us (235 MB at 5.7 TB/s; a large copy moves 5.2), 32
+// tokens 42.8, 64 tokens (64 x 64 tiles) 44.4.  More are bound by the matrix cores and LDS: 256 tokens (128 x 128) 70 us, 860 TFLOP/s.
 //
 // Stages of 128 K bytes of the tile's 2 BF rows of W (BF of Wg, BF of Wu) and BT rows of X travel straight into a ring of NS
 // slots in LDS; rows are eight 16-byte chunks, XOR-swizzled as in gemm_mfma.hpp.  The fragments of a stage are read from LDS behind
