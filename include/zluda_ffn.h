@@ -76,7 +76,7 @@ typedef struct zluda_ffn_gated_grad {
 } zluda_ffn_gated_grad;
 
 uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void *workspace, size_t workspace_size, void *stream);
-/* (of the structure's sizes, types and which matrices are present; pointers are only compared with NULL) */
+/* (of the structure's sizes, types, pitches and which matrices are present; pointers are only compared with NULL) */
 uint32_t zluda_ffn_gated_backward_workspace(const zluda_ffn_gated_grad *p, size_t *bytes);
 
 /* Layer norm over rows: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(variance + eps), the variance that of the row
