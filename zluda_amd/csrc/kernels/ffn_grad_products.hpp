@@ -9,6 +9,11 @@
 // fragments of the one arrive while the products of the other run.  The barrier lies between them: behind it stage kt + 1 has landed and every
 // wave has the fragments of stage kt, whose slot takes stage kt + 2.  Two workgroups share a CU, and one computes while the other waits.
 //
+// Bound by the matrix cores and LDS where there are many tiles (8192 tokens, 2048 x 8192: 1040 us, 1.06 PFLOP/s; that is where tiles of 256 x 256, one
+// product after the other, take 810), by the round trips of a stage's requests and the last tiles where there are few (1001 tokens, 1024 x 2816:
+// 34 us, MFMAs 42 % of the time).  Tiles of 256 x 256 here, eight waves, have no registers left for the offsets of dZ's rows: 700 tokens, 4096 x 14336 381 us
+// at best against 383, 1500, 2048 x 8192 235 against 229.
+//
 // K rows past the end are requested out of the buffer windows' range and become zeros; every wait is for everything in flight, so that it does not
 // matter in which order such requests retire.  (Whole stages past the end requested like that cost 7 % at three stages, 150 tokens.)
 #pragma once
