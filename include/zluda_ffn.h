@@ -34,7 +34,11 @@ extern "C" {
  * |v| <= 448 * 2^e for every finite v of the 32, and at least -126; scales holds e + 127 (UE8M0) at
  * scales[r * ld_scales + c / 32].  data holds the OCP E4M3 code of v / 2^e, rounded to nearest, ties to even; what is not
  * finite is stored as NaN (of either sign) and does not count for e.  ld is a multiple of 32 and data is 16-byte aligned; a row's last block
- * is filled up with zeros, so that rows hold 32 * ceil(columns / 32) codes.  ld_scales >= ceil(columns / 32). */
+ * is filled up with zeros, so that rows hold 32 * ceil(columns / 32) codes.  ld_scales >= ceil(columns / 32).
+ *
+ * Rounding to E4M3 can take a finite value near the top of its type to the power of two behind it, 65536 for 16F (from 63488 on), 2^128 for 16BF and
+ * 32F: checkpoint_load rounds that to the type, which makes it an infinity; what the backward passes read of a checkpoint counts as the largest finite
+ * number there (x of the gated layer of its type, the others of 32F), so that only what was not finite spoils a sum. */
 typedef struct zluda_ffn_matrix {
   void *data;
   void *scales;      /* checkpoints only */

@@ -9,10 +9,12 @@ typedef uint32_t ffn_u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t ffn_u2 __attribute__((ext_vector_type(2)));
 
 // ---- elements -------------------------------------------------------------------------------------------------------------
-// Raw8: eight elements as they lie in memory.
+// Raw8: eight elements as they lie in memory.  top: the bits of the largest finite element, as 32F; top_scale: the scale byte of a checkpoint's block
+// from which on a value can lie beyond it.
 struct ElemBF16 {
   using raw = uint16_t;
   static constexpr uint32_t type = CUDA_R_16BF;
+  static constexpr uint32_t top = 0x7f7f0000u, top_scale = 247;
   struct Raw8 { uint32_t w[4]; };
   static __device__ __forceinline__ float dec(raw v) { return dec_bf16(v); }
   static __device__ __forceinline__ raw enc(float v) { return enc_bf16(v); }
@@ -22,6 +24,7 @@ struct ElemBF16 {
 struct ElemF16 {
   using raw = uint16_t;
   static constexpr uint32_t type = CUDA_R_16F;
+  static constexpr uint32_t top = 0x477fe000u, top_scale = 135;
   struct Raw8 { uint32_t w[4]; };
   static __device__ __forceinline__ float dec(raw v) { return dec_f16(v); }
   static __device__ __forceinline__ raw enc(float v) { return enc_f16(v); }
@@ -31,6 +34,7 @@ struct ElemF16 {
 struct ElemF32 {
   using raw = float;
   static constexpr uint32_t type = CUDA_R_32F;
+  static constexpr uint32_t top = 0x7f7fffffu, top_scale = 247;
   struct Raw8 { uint32_t w[8]; };
   static __device__ __forceinline__ float dec(raw v) { return v; }
   static __device__ __forceinline__ raw enc(float v) { return v; }
@@ -194,6 +198,20 @@ __device__ __forceinline__ void ckpt_get8(const Ckpt8 &c, float (&v)[8]) {
   const float s = ckpt_scale(c.scale);
   ckpt_decode4(c.codes[0], s, v);
   ckpt_decode4(c.codes[1], s, v + 4);
+}
+// The same for an operand of the type E, with values beyond its largest as that one.  (A block's scale is the smallest under which nothing is above 448, but
+// rounding takes what lies in [248, 256) times the scale to 256 times: from the last 1/32 of a type's last binade to the power of two behind it.  One such
+// infinity in X would be a whole column of dW.)  NaN stays.  The blocks that can hold such values are a branch that hardly a wave takes.
+template <class E>
+__device__ __forceinline__ void ckpt_finite8(float (&v)[8]) {
+  const float top = bits2f(E::top);
+#pragma unroll
+  for (int e = 0; e < 8; e++) v[e] = v[e] > top ? top : v[e] < -top ? -top : v[e];
+}
+template <class E>
+__device__ __forceinline__ void ckpt_get8_finite(const Ckpt8 &c, float (&v)[8]) {
+  ckpt_get8(c, v);
+  if (__builtin_expect(c.scale >= E::top_scale, 0)) ckpt_finite8<E>(v);
 }
 
 // ---- sums over lanes --------------------------------------------------------------------------------------------------------

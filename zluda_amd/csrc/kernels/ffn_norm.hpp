@@ -210,7 +210,7 @@ __global__ __launch_bounds__(T *R) void norm_backward_kernel(NormGradParams p) {
 #pragma unroll
     for (int i = 0; i < NV; i++) {
       if constexpr (CK) {
-        ckpt_get8(q.x[i], x[i]);
+        ckpt_get8_finite<ElemF32>(q.x[i], x[i]);
       } else {
 #pragma unroll
         for (int e = 0; e < 8; e++) x[i][e] = E::get(q.x[i], e);
