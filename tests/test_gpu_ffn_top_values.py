@@ -1,4 +1,4 @@
-"""Checkpoints of values near the type's largest.  E4M3 rounds the top 1/32 of a block's last binade up to the next power of two, so a finite value may
+"""Checkpoints of values near the type's largest.  E4M3 rounds [248, 256) times a block's scale up to 256 times, so a finite value may
 stand there as 65536 (f16) or 2^128 (bf16, f32), which the type does not have.  What the backward passes read stays finite: such a value counts as
 the largest one, and only what was not finite is NaN."""
 import pytest

@@ -200,7 +200,7 @@ __device__ __forceinline__ void ckpt_get8(const Ckpt8 &c, float (&v)[8]) {
   ckpt_decode4(c.codes[1], s, v + 4);
 }
 // The same for an operand of the type E, with values beyond its largest as that one.  (A block's scale is the smallest under which nothing is above 448, but
-// rounding takes what lies in [248, 256) times the scale to 256 times: from the last 1/32 of a type's last binade to the power of two behind it.  One such
+// rounding takes what lies in [248, 256) times the scale to 256 times: from the last 1/32 of a type's range to the power of two behind it.  One such
 // infinity in X would be a whole column of dW.)  NaN stays.  The blocks that can hold such values are a branch that hardly a wave takes.
 template <class E>
 __device__ __forceinline__ void ckpt_finite8(float (&v)[8]) {
