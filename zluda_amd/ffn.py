@@ -11,6 +11,7 @@ A call object is configured once with a plain dict (types, sizes, pitches) and r
   NormBackward   the same; x_kept (KEPT_PLAIN or KEPT_8BIT), add (bool), weights (bool: dweight and dbias, default True)
   Checkpoint     type, rows, cols
 
+A call object writes the addresses into its own structure and hands that to the library: one thread at a time may run it (several threads: an object each).
 `workspace` is the number of bytes of device scratch that run() wants.  Pitches default to tight rows, those of checkpoints to what
 checkpoint_buffers() makes: codes padded to 32 columns, one scale byte for each 32.  A status other than 0 raises CublasLtError.
 """
@@ -138,9 +139,7 @@ class GatedForward(_Call):
     def run(self, x, w, h, bias=None, gate=None, gate_scales=None, up=None, up_scales=None, workspace=None, workspace_size=0, stream=None):
         mx, mw, mh, mg, mu = self._m
         mx.data, mw.data, mh.data, self.p.bias = x, w, h, bias
-        mg.data, mu.data = gate, up
-        if gate_scales is not None:
-            mg.scales, mu.scales = gate_scales, up_scales
+        mg.data, mg.scales, mu.data, mu.scales = gate, gate_scales, up, up_scales
         status = self._call(self._ref, workspace, workspace_size, stream)
         if status:
             _check(status, "zluda_ffn_gated_forward")
