@@ -6,18 +6,15 @@
 #include <cstring>
 
 #include "../../include/zluda_gemm_launch.h"
-#include "ffn_launch.hpp"
+#include "ffn_launchers.hpp"
 #include "kernels/ffn_elementwise.hpp"
 #include "kernels/ffn_norm.hpp"
-#include "kernels/store_window.hpp"
 #include "planner.hpp"
 
 using namespace zluda_amd;
 
 namespace {
 
-constexpr uint64_t kMaxSide = 0x7fffff00;             // sizes are 32-bit numbers inside the kernels, with room to round up
-constexpr uint64_t kMaxFeatures = 1 << 20;            // (2^15 blocks of 32 along a grid's second dimension)
 // Split-K partial tiles of the backward pass's matmuls.  With twice as much the planner splits further than pays here (1001 tokens, 1024 x
 // 2816: dx 24.0 us, 27.9 with 32 MiB, 29.1 with 8; 500, 4096 x 11008: 118, 122, 203).
 constexpr uint64_t kGemmWorkspace = 16ull << 20;
@@ -75,68 +72,6 @@ uint32_t check_forward(const zluda_ffn_gated *p) {
   return CUBLAS_STATUS_SUCCESS;
 }
 
-// The matmul kernels reach an operand through a window of 2 GiB.  Rows of one of pitch `ld` (16-bit elements) that lie inside one, what a kernel
-// asks for past their end included; all of them where they are wider apart than that helps.  A call of more rows is run in parts of
-// so many (40000 tokens, 2048 x 16384: dX 187 ms on the kernel without a window, 5.1 in two parts, dW 203 and 5.6; forward 300000 tokens,
-// 4096 x 1024: 3.6 ms, 1390 TFLOP/s).
-uint64_t rows_in_window(uint64_t rows, int64_t ld) {
-  const int64_t most = ld < 1 ? 0 : (0x3fffffffll / ld - 256) & ~255ll;  // (a workspace is asked for before pitches are checked)
-  return most > 0 && rows > (uint64_t)most ? (uint64_t)most : rows;
-}
-bool in_window(uint64_t rows, int64_t ld) { return (int64_t)(rows + 256) <= 0x3fffffffll / ld; }
-
-// dX and dW in one launch of 128 x 128 tiles (kernels/ffn_grad_products.hpp), or one after the other on the framework's matmul kernels?  Together, us
-// of whole backward passes and in brackets one after the other: 64 tokens, 4096 x 14336 118 (167), 300, 2048 x 5632 59 (70), 700, 4096 x 14336
-// 399 (451), 1100 594 (663), 1001, 1024 x 2816 46 (55), 1500, 2048 x 8192 238 (270), 5000, 1024 x 8192 388 (465), 3000, 4096 x 2816 284 (286).
-// One after the other
-//  * where both fill the chip by themselves, dW twice with tiles of 256 x 256, which compute faster (2000, 4096 x 11008 758 and 709; 8192, 2048 x
-//    8192 1152 and 925);
-//  * where a tile of dW alone takes more than twice the time all tiles take the chip: its K is not shared out here (8192, 1024 x 512 105 and 60;
-//    3000, 512 x 512 38 and 33; with as much as twice 4096, 1024 x 1024 61 and 64, 8192, 512 x 2048 148 and 131).
-struct GradTogether {
-  uint32_t splits, split_stages;  // shares of dX's K; 0: one after the other
-  uint64_t part;                  // bytes of their sums
-};
-// Stages until the launch is done, of `slots` workgroups at a time that take dX's n_dx * s shares, then the tiles of dW: half way between an even load
-// and one workgroup after the other at an even pace (one without a neighbour is faster, but not by as much).  A tile's start and end are as
-// long as three stages; a stage of a share takes `pace` quarters more than one at an even load, as it waits for W; the shares' sums are written and
-// read again, in a launch of their own.  Measured, us, shares of dX and times: 1001, 1024 x 2816 1: 71, 2: 49, 3: 46, 4: 49, 8: 49; 300, 2048 x 5632 3: 60,
-// 5: 56, 8: 57; 700, 4096 x 14336 1: 459, 2: 393, 3: 415; 2000, 1024 x 1024 1: 32, 2: 41; W from memory: 150, 4096 x 14336 3: 195, 5: 169, 8: 168, 12: 176;
-// 64, 4096 x 14336 3: 181, 8: 118, 12: 131; 100, 5120 x 13824 3: 198, 5: 164, 8: 168.
-double grad_together_stages(uint64_t slots, uint64_t n_dx, uint64_t k_dx, uint64_t n_dw, uint64_t k_dw, uint64_t s, uint64_t pace) {
-  const uint64_t l1 = (k_dx + s - 1) / s + 3, l2 = k_dw + 3, n1 = n_dx * s, even = (n1 * l1 + n_dw * l2) / slots, rounds = n1 / slots, rest = n1 % slots;
-  uint64_t low = std::max(even, rounds * l1 + (rest ? l1 + l1 * pace / 4 : 0)), high = low + l1 + (n_dw / slots + 2) * l2;  // (dW's tiles fit behind `high`)
-  while (low < high) {
-    const uint64_t end = (low + high) / 2, early = end > rounds * l1 ? (end - rounds * l1) / l2 : 0, late = end > (rounds + 1) * l1 ? (end - (rounds + 1) * l1) / l2 : 0;
-    if ((slots - rest) * early + rest * late >= n_dw) high = end;
-    else low = end + 1;
-  }
-  return 0.5 * (double)(even + low) + (s > 1 ? 5.0 + 0.04 * (double)n1 : 0.0);
-}
-GradTogether grad_together(const zluda_ffn_gated_grad *p) {
-  GradTogether g{0, 0, 0};
-  if (!p->dx.data || !p->dw.data || !p->tokens || p->model % 8 || p->features % 4) return g;
-  auto tiles = [](uint64_t a, uint64_t b, uint64_t side) { return ((a + side - 1) / side) * ((b + side - 1) / side); };
-  const uint64_t f2 = 2 * p->features, slots = 2 * (uint64_t)cus(), n_dx = tiles(p->model, p->tokens, kGradTile), n_dw = tiles(p->model, f2, kGradTile);
-  const uint64_t k_dx = (f2 + kGradStage - 1) / kGradStage, k_dw = (p->tokens + kGradStage - 1) / kGradStage;
-  const uint64_t all = (n_dx * k_dx + n_dw * k_dw + slots - 1) / slots;  // stages of a workgroup if they were shared out evenly
-  if ((n_dx >= slots && tiles(p->model, f2, 256) >= slots) || k_dw > 2 * all) return g;
-  const uint64_t pace = 8 * p->features * p->model > 256ull << 20 ? 2 : 1;  // (W and dW are more than the memory-side cache)
-  uint64_t want = 1;
-  double best = 0.0;
-  for (uint64_t n = 1; n <= std::min<uint64_t>(16, k_dx); n++) {
-    const double stages = grad_together_stages(slots, n_dx, k_dx, n_dw, k_dw, n, pace);
-    if (n == 1 || stages < best) {
-      want = n;
-      best = stages;
-    }
-  }
-  g.split_stages = (uint32_t)((k_dx + want - 1) / want);
-  g.splits = (uint32_t)((k_dx + g.split_stages - 1) / g.split_stages);
-  g.part = g.splits > 1 ? g.splits * n_dx * kGradTile * kGradTile * 4 : 0;
-  return g;
-}
-
 // where the parts of the backward pass's workspace lie
 struct GradPlan {
   uint64_t dz, x, sums, gemm, acc, total;  // offsets
@@ -150,7 +85,7 @@ struct GradPlan {
 // workgroups a CU that walk the rows); with them at least four rows a thread and at most eight workgroups a CU, because each
 // leaves a row of partial sums (1001 x 2816: 10.9 us, 15.4 with one row a thread).
 uint32_t grad_shares(uint64_t tokens, uint64_t features, bool sums) {
-  const uint64_t strips = (features + 511) / 512, each = sums ? 16 : 4, most = std::max<uint64_t>(1, (tokens + each - 1) / each);
+  const uint64_t strips = column_strips(features), each = sums ? 16 : 4, most = std::max<uint64_t>(1, (tokens + each - 1) / each);
   const uint64_t want = sums ? std::max<uint64_t>(1, ((uint64_t)cus() * 8 + strips - 1) / strips) : most;
   return (uint32_t)std::min<uint64_t>({want, most, kGridY});
 }
@@ -165,7 +100,7 @@ GradPlan grad_plan(const zluda_ffn_gated_grad *p) {
   uint64_t at = 0;
   g.lddz = p->dz.data ? p->dz.ld : aligned_pitch(2 * p->features);
   g.shares = grad_shares(p->tokens, p->features, p->dbias != nullptr);
-  g.together = grad_together(p);
+  g.together = grad_together(p, cus());
   g.dz = at;
   if (!p->dz.data) at += aligned256(p->tokens * (uint64_t)g.lddz * 2);
   g.x = at;
@@ -207,7 +142,7 @@ uint32_t check_backward(const zluda_ffn_gated_grad *p) {
 
 template <class E>
 uint32_t launch_checkpoint(bool store, const CheckpointParams &p, hipStream_t s) {
-  const dim3 grid((p.cols + 511) / 512, (uint32_t)std::min<int64_t>((p.rows + 3) / 4, kGridY));
+  const dim3 grid(column_strips(p.cols), (uint32_t)std::min<int64_t>((p.rows + 3) / 4, kGridY));
   return store ? launch_kernel(checkpoint_store_kernel<E>, grid, dim3(256), s, p) : launch_kernel(checkpoint_load_kernel<E>, grid, dim3(256), s, p);
 }
 
@@ -232,7 +167,7 @@ uint32_t checkpoint_call(bool store, uint64_t rows, uint64_t cols, const zluda_f
 
 template <class E, bool CK>
 uint32_t launch_gated_grad(const GatedGradParams &g, uint32_t shares, hipStream_t s) {
-  const dim3 grid((g.features + 511) / 512 + (g.load.x ? (g.load.cols + 511) / 512 : 0), shares);
+  const dim3 grid(column_strips(g.features) + (g.load.x ? column_strips(g.load.cols) : 0), shares);
   switch (g.activation) {
   case ZLUDA_FFN_SILU: return launch_kernel(gated_grad_kernel<E, CK, 0>, grid, dim3(256), s, g);
   case ZLUDA_FFN_GELU: return launch_kernel(gated_grad_kernel<E, CK, 1>, grid, dim3(256), s, g);
@@ -261,12 +196,10 @@ uint32_t run_matmul(uint32_t type, uint32_t transa, uint32_t transb, uint64_t m,
   q.A = A; q.B = B; q.C = D; q.D = D;
   q.workspace = ws; q.workspace_size = ws_size;
   zluda_gemm_plan plan;
-  // Tiles of 256 x 256 wherever they fill the chip twice; the planner's own choice, made from the time of a single stage, takes half-size ones
-  // for some of these (A:N B:T 2360 x 15440 x 6196, 610 tiles: 443 us on them, 557 on 128 x 128).
   static_assert(kTrVariants[3].bp == 256 && kTrVariants[3].bq == 256, "the largest tile");
   const uint32_t cu = zluda_gemm_device_cu_count();
   uint32_t st = CUBLAS_STATUS_NOT_SUPPORTED;
-  if (((m + 255) / 256) * ((n + 255) / 256) >= 2ull * cu) st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_MFMA_TR16, 3, cu, &plan);
+  if (grad_largest_tiles(m, n, cu)) st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_MFMA_TR16, 3, cu, &plan);
   if (st != CUBLAS_STATUS_SUCCESS) st = zluda_gemm_plan_problem(&q, ZLUDA_KERNEL_AUTO, -1, cu, &plan);
   if (st == CUBLAS_STATUS_SUCCESS) st = zluda_gemm_launch(&q, &plan, s);
   return st;
@@ -278,15 +211,8 @@ uint32_t zero_rows(void *p, uint64_t rows, uint64_t row_bytes, int64_t pitch_byt
 }
 
 uint32_t round_rows(uint32_t type, const RoundParams &r, hipStream_t s) {
-  const dim3 grid((uint32_t)((r.cols + 511) / 512), (uint32_t)std::min<int64_t>((r.rows + 3) / 4, kGridY));
+  const dim3 grid(column_strips(r.cols), (uint32_t)std::min<int64_t>((r.rows + 3) / 4, kGridY));
   return type == CUDA_R_16BF ? launch_kernel(round_rows_kernel<ElemBF16>, grid, dim3(256), s, r) : launch_kernel(round_rows_kernel<ElemF16>, grid, dim3(256), s, r);
-}
-
-// 16-byte pieces of all operands and results, through windows of 2 GiB
-bool grad_together_operands(const zluda_ffn_gated_grad *p, const zluda_ffn_matrix &x, const GradPlan &plan, const void *dz) {
-  return !((p->w.ld | x.ld | plan.lddz | p->dx.ld | p->dw.ld) & 7) && p->dx.ld < kNarrowPitch && p->dw.ld < kNarrowPitch &&
-         !(((uintptr_t)p->w.data | (uintptr_t)x.data | (uintptr_t)dz | (uintptr_t)p->dx.data | (uintptr_t)p->dw.data) & 15) && in_window(p->tokens, x.ld) &&
-         in_window(p->tokens, plan.lddz) && in_window(2 * p->features, p->w.ld);
 }
 
 // the two products and the bias gradient in one launch, then the sums of dX's shares
@@ -450,7 +376,7 @@ extern "C" uint32_t zluda_ffn_gated_backward(const zluda_ffn_gated_grad *p, void
   FFN_CHECK(type == CUDA_R_16BF ? (ck ? launch_gated_grad<ElemBF16, true>(g, plan.shares, s) : launch_gated_grad<ElemBF16, false>(g, plan.shares, s))
                                 : (ck ? launch_gated_grad<ElemF16, true>(g, plan.shares, s) : launch_gated_grad<ElemF16, false>(g, plan.shares, s)));
   void *gemm_ws = ws + plan.gemm;
-  if (plan.together.splits && grad_together_operands(p, x, plan, g.dz)) return run_together(type, p, x, plan, g, (float *)gemm_ws, s);
+  if (plan.together.splits && grad_together_operands(p, x, plan.lddz, g.dz)) return run_together(type, p, x, plan, g, (float *)gemm_ws, s);
   if (p->dbias) {
     NormFinishParams f{g.part, p->dbias, nullptr, (int32_t)plan.shares, (int32_t)(2 * p->features), type};
     FFN_CHECK(launch_kernel(norm_finish_kernel<16, 64>, dim3((uint32_t)((2 * p->features + 15) / 16), 1), dim3(1024), s, f));

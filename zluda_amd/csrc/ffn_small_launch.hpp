@@ -2,7 +2,7 @@
 #pragma once
 #include <cstring>
 
-#include "ffn_launch.hpp"
+#include "ffn_launchers.hpp"
 #include "kernels/ffn_gated_any.hpp"
 #include "kernels/ffn_gated_tile.hpp"
 

@@ -17,7 +17,7 @@
 // K rows past the end are requested out of the buffer windows' range and become zeros; every wait is for everything in flight, so that it does not
 // matter in which order such requests retire.  (Whole stages past the end requested like that cost 7 % at three stages, 150 tokens.)
 #pragma once
-#include "../ffn_launch.hpp"
+#include "../ffn_launchers.hpp"
 #include "ffn_gated_any.hpp"
 #include "gemm_mfma_pipe16.hpp"
 
