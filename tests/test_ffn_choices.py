@@ -2,7 +2,8 @@
 CUs, so that a new time or tile in the rules cannot leave one of them without a test."""
 import test_gpu_ffn
 import test_gpu_ffn_persistent
-from ffn_probe import gated_tile, tile_shape
+import test_gpu_ffn_products
+from ffn_probe import gated_tile, grad_splits, tile_shape
 
 
 def sizes(test, names="t,d,f"):
@@ -30,3 +31,20 @@ def test_the_wide_tiles_sizes_cover_their_loops():
     assert any(n <= 256 for n in tiles) and any(n > 512 for n in tiles) and any(256 < n < 512 for n in tiles)
     assert {-(-d // 64) for _, d, _ in test_gpu_ffn_persistent.SIZES} == {1, 2, 3, 4, 6}
     assert all(t % t0 for t, _, _ in test_gpu_ffn_persistent.SIZES) and any(f % f0 and f % 2 for _, _, f in test_gpu_ffn_persistent.SIZES)
+
+
+def test_the_launch_of_both_products_has_tests_of_its_loops():
+    """stages of dW's K, shares of dX's K and stages of a share, tiles of tokens"""
+    chosen = {s: grad_splits(*s) for s in test_gpu_ffn_products.SIZES}
+    assert all(n > 0 for n, _ in chosen.values())
+    assert {n for n, _ in chosen.values()} >= {1, 2, 3, 4, 5, 6, 10, 13, 16}
+    assert {-(-t // 64) for t, _, _ in chosen} >= {3, 4, 5, 6, 7, 8, 10, 11, 16} and any(t % 64 == 1 for t, _, _ in chosen)
+    assert {-(-t // 128) for (t, _, _), (n, _) in chosen.items() if n > 1} >= {2, 3, 4, 5, 8}
+    # a last share that is shorter than the others, one of a single stage less, shares of 4 stages and of many
+    stages = {s: -(-2 * s[2] // 64) for s in chosen}
+    assert any(n > 1 and stages[s] % each for s, (n, each) in chosen.items()) and {each for _, each in chosen.values()} >= {4, 5, 6, 7, 8, 9, 16}
+    for pad in (0, 8):
+        for x_kept in (False, True):
+            for s in chosen:
+                for dz_ld in (None, 2 * s[2] + pad):
+                    assert grad_splits(*s, pad=pad, skip=pad, dz_ld=dz_ld, x_kept=x_kept) == chosen[s]
