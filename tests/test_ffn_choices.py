@@ -1,9 +1,13 @@
 """The GPU tests of the feed-forward operators reach every kernel that a call can take: the launches' rules replayed over the tests' sizes on a chip of 256
 CUs, so that a new time or tile in the rules cannot leave one of them without a test."""
+import ffn_probe
 import test_gpu_ffn
+import test_gpu_ffn_large_tiles
 import test_gpu_ffn_persistent
 import test_gpu_ffn_products
 from ffn_probe import gated_tile, grad_splits, tile_shape
+from planner_probe import planned
+from zluda_amd import abi as K
 
 
 def sizes(test, names="t,d,f"):
@@ -48,3 +52,13 @@ def test_the_launch_of_both_products_has_tests_of_its_loops():
             for s in chosen:
                 for dz_ld in (None, 2 * s[2] + pad):
                     assert grad_splits(*s, pad=pad, skip=pad, dz_ld=dz_ld, x_kept=x_kept) == chosen[s]
+
+
+def test_the_largest_tiles_have_tests_and_are_planned(api):
+    """dx: A:N B:N, model x tokens, K 2 features; dw: A:N B:T, model x 2 features, K tokens"""
+    for which, t, d, f, _ in test_gpu_ffn_large_tiles.CASES:
+        m, n, k, tb = (d, t, 2 * f, 0) if which == "dx" else (d, 2 * f, t, 1)
+        assert ffn_probe.load().probe_grad_largest_tiles(m, n, 256)
+        status, _, plan, _ = planned(api, m, n, k, ta=0, tb=tb, workspace=16 << 20, family=K.ZLUDA_KERNEL_MFMA_TR16, variant=3)
+        assert status == 0 and (plan.kernel, plan.variant) == (K.ZLUDA_KERNEL_MFMA_TR16, 3)
+    assert not ffn_probe.load().probe_grad_largest_tiles(4096, 31 * 256, 256) and ffn_probe.load().probe_grad_largest_tiles(4096, 31 * 256 + 1, 256)
