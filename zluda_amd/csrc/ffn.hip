@@ -15,8 +15,9 @@ using namespace zluda_amd;
 
 namespace {
 
-// Split-K partial tiles of the backward pass's matmuls.  With twice as much the planner splits further than pays here (1001 tokens, 1024 x
-// 2816: dx 24.0 us, 27.9 with 32 MiB, 29.1 with 8; 500, 4096 x 11008: 118, 122, 203).
+// Split-K partial tiles of the matmuls that make dX and dW one after the other, or one of them alone.  With twice as much the planner splits further than pays
+// here, with half as much not far enough.  Whole backward passes, us, with 16, 32 and 8 MiB: dX alone, 1001 tokens, 1024 x 2816 30.8, 33.9, 34.9; 500, 4096 x
+// 11008 108, 115, 164; dW alone, 8192, 1024 x 512 37.0, 40.5, 45.5; both, 8192, 1024 x 512 61.9, 64.3, 67.3; 1500, 1023 x 4000 98, 96, 122; 3000, 512 x 512 32.2, 32.2, 29.0.
 constexpr uint64_t kGemmWorkspace = 16ull << 20;
 constexpr int kGridY = 65535;
 

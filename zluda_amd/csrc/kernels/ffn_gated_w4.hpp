@@ -1,5 +1,5 @@
 // The gated feed-forward products on the persistent four-wave kernel (gemm_mfma_w4.hpp, W4_EPI_GATED): 128 features and 256
-// tokens a tile, 64 features of Wg and the same 64 of Wu in a wave's 128 rows.
+// or 192 tokens a tile, 64 features of Wg and the same 64 of Wu in a wave's 128 rows.
 //
 // Bound by the matrix cores, as the plain product of X and [Wg; Wu]; the activation, the product and what is kept ride in the
 // epilogue, from the accumulators, while the next tile's first stages are in flight.

@@ -1,6 +1,6 @@
 """The feed-forward half of a transformer block on this library's operators, forward and backward:
 
-    out = r + act(n Wg^T) * (n Wu^T) Wd^T,   n = norm(r)
+    out = r + (act(n Wg^T) * (n Wu^T)) Wd^T,   n = norm(r)
 
 norm and the gated products through zluda_amd.ffn, the down projection and its two gradients through cublasLtMatmul (the residual is its
 C, with beta 1).  `keep8` keeps what the backward pass needs -- r, n, G and U -- as 8-bit checkpoints; H is computed again from G and U.
