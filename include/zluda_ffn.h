@@ -2,6 +2,8 @@
  * zluda_ffn.h -- what stands beside the matmuls in the feed-forward half of a transformer block: a gated feed-forward layer,
  * the layer norm in front of it, and activation checkpoints in 8 bits, which the forward passes of both write and the
  * backward passes read.  The down projection is an ordinary cublasLtMatmul.  The reference has no counterpart.
+ * For layers in 8 bits and for layers of experts: RMS norm with the residual's addition, packing of activations and weights with a scale for
+ * each 128 (the operands of a cublasLtMatmul with such scales), and products grouped by expert.
  *
  * Conventions of the library: plain pointers to device memory, sizes and enum numbers in, a cublasStatus_t out; work is
  * enqueued on `stream` (a hipStream_t) and nothing is allocated, synchronised or kept; all calls may be captured into a
@@ -38,12 +40,20 @@ extern "C" {
  *
  * Rounding to E4M3 can take a finite value near the top of its type to the power of two behind it, 65536 for 16F (from 63488 on), 2^128 for 16BF and
  * 32F: checkpoint_load rounds that to the type, which makes it an infinity; what the backward passes read of a checkpoint counts as the largest finite
- * number there (x of the gated layer of its type, the others of 32F), so that only what was not finite spoils a sum. */
+ * number there (x of the gated layer of its type, the others of 32F), so that only what was not finite spoils a sum.
+ *
+ * type CUDA_R_8F_E4M3 where an operator below says "packed": data holds E4M3 codes, scales floats.  Each 128 neighbours of a row (of a weight:
+ * each block of 128 rows and 128 columns) share a scale s, the largest finite magnitude of them divided by 448, and at least 2^-126; the
+ * code is that of v / s, rounded to nearest, ties to even; what is not finite is stored as NaN and does not count for s.  The scale of
+ * element (r, c) is at scales[c / 128 * ld_scales + r], ld_scales >= rows (blocks of 128 rows: at scales[r / 128 * ld_scales + c / 128],
+ * ld_scales >= ceil(columns / 128)): with ld_scales the rows what CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F takes, with
+ * ceil(columns / 128) rounded up to four what BLK128x128_32F takes.  data may lie anywhere (rows on 16 bytes are the fast case); nothing behind a
+ * row's last column is written. */
 typedef struct zluda_ffn_matrix {
   void *data;
-  void *scales;      /* checkpoints only */
+  void *scales;      /* checkpoints and what is packed */
   int64_t ld;        /* elements */
-  int64_t ld_scales; /* bytes; checkpoints only */
+  int64_t ld_scales; /* bytes, of a checkpoint; floats, of what is packed */
   uint32_t type;     /* cudaDataType */
 } zluda_ffn_matrix;
 
@@ -118,6 +128,82 @@ uint32_t zluda_ffn_norm_backward_workspace(const zluda_ffn_norm_grad *p, size_t 
 /* rows x cols between a plain matrix and a checkpoint. */
 uint32_t zluda_ffn_checkpoint_store(uint64_t rows, uint64_t cols, const zluda_ffn_matrix *x, const zluda_ffn_matrix *checkpoint, void *stream);
 uint32_t zluda_ffn_checkpoint_load(uint64_t rows, uint64_t cols, const zluda_ffn_matrix *checkpoint, const zluda_ffn_matrix *x, void *stream);
+
+/* Root-mean-square norm over rows, behind the residual's addition:
+ *   h = x + residual, rounded once to the type (residual absent: h = x);  rstd = 1 / sqrt(mean(h^2) + eps);  y = h * rstd * weight
+ * The norm takes the rounded h, which is what the backward pass reads.  x, residual, sum (receives h), y: rows x cols of one type (16F, 16BF, 32F), cols up
+ * to 16384; packed receives y packed, from its 32-bit values; sum, y and packed are absent or wanted (data == NULL), one of them at least wanted;
+ * weight: cols elements of weight_type (x's or 32F), NULL: 1; rstd: rows floats or NULL.  sum or y may be x or residual itself, with its
+ * pitch, but sum is not y. */
+typedef struct zluda_ffn_rms {
+  uint64_t rows, cols;
+  float eps;
+  uint32_t weight_type;
+  zluda_ffn_matrix x, residual, sum, y, packed;
+  const void *weight;
+  float *rstd;
+} zluda_ffn_rms;
+
+uint32_t zluda_ffn_rms_forward(const zluda_ffn_rms *p, void *stream);
+
+/* The gradients, with xhat = h * rstd:
+ *   dx = rstd * (dy * weight - xhat * mean_c(dy * weight * xhat)) + add     (of x, and of residual)
+ *   dweight = sum over rows of dy * xhat   (weight_type; the order of the sum is fixed)
+ * add, dx and dweight may be absent, dx and dweight not both; dx may be add or dy itself, with its pitch. */
+typedef struct zluda_ffn_rms_grad {
+  uint64_t rows, cols;
+  uint32_t weight_type;
+  zluda_ffn_matrix h, dy, add, dx;
+  const void *weight;
+  const float *rstd;
+  void *dweight;
+} zluda_ffn_rms_grad;
+
+uint32_t zluda_ffn_rms_backward(const zluda_ffn_rms_grad *p, void *workspace, size_t workspace_size, void *stream);
+uint32_t zluda_ffn_rms_backward_workspace(const zluda_ffn_rms_grad *p, size_t *bytes);
+
+/* h = act(gate) * up, or act(gate) where up is absent; ZLUDA_FFN_COPY: h = gate (up absent).  gate, up, y: rows x cols of one type (16F, 16BF, 32F);
+ * y and packed receive h (either may be absent), the packed one from the 32-bit values, with scales for 128 of a row (block_rows 1) or for blocks of
+ * 128 x 128 (block_rows 128).  gate and up may be the halves of one matrix.  y may be gate or up itself, with its pitch. */
+#define ZLUDA_FFN_COPY 3u
+typedef struct zluda_ffn_activation {
+  uint32_t activation, block_rows;
+  uint64_t rows, cols;
+  zluda_ffn_matrix gate, up, y, packed;
+} zluda_ffn_activation;
+
+uint32_t zluda_ffn_activate(const zluda_ffn_activation *p, void *stream);
+
+/* What is packed, as plain values: code times scale, rounded to y's type (a value beyond its largest is that one). */
+uint32_t zluda_ffn_unpack(uint64_t rows, uint64_t cols, uint32_t block_rows, const zluda_ffn_matrix *packed, const zluda_ffn_matrix *y, void *stream);
+
+/* Products grouped by expert.  Rows are sorted by expert: those of expert e are offsets[e] .. offsets[e + 1] - 1, offsets being experts + 1 numbers in device
+ * memory that do not decrease, from 0 to rows; an expert may have none, and rows that no expert has stay as they are in y and dx.
+ *   y[r] = W_e x[r]      x: rows x model, w: experts * features x model (expert e: rows e * features and on), y: rows x features
+ * x, w and y of one 16-bit type; or x packed, w packed in blocks of 128 x 128 that start anew at each expert (scales of expert e from block row
+ * e * ceil(features / 128) on), and y 16F, 16BF or 32F.  Sums in 32 bits.  Numbers in offsets that break the rule give wrong results, but nothing outside
+ * the matrices is touched. */
+#define ZLUDA_FFN_MAX_EXPERTS 4096u
+typedef struct zluda_ffn_grouped {
+  uint64_t rows, experts, features, model;
+  const int32_t *offsets;
+  zluda_ffn_matrix x, w, y;
+} zluda_ffn_grouped;
+
+uint32_t zluda_ffn_grouped_forward(const zluda_ffn_grouped *p, void *workspace, size_t workspace_size, void *stream);
+uint32_t zluda_ffn_grouped_forward_workspace(const zluda_ffn_grouped *p, size_t *bytes);
+
+/* The gradients, all matrices of one 16-bit type:
+ *   dx[r] = W_e^T dy[r] (rows x model)      dw: dW_e = sum over the rows of e of dy[r]^T x[r] (experts * features x model), zeros for an expert without rows
+ * dx or dw may be absent; w is needed for dx, x for dw. */
+typedef struct zluda_ffn_grouped_grad {
+  uint64_t rows, experts, features, model;
+  const int32_t *offsets;
+  zluda_ffn_matrix dy, x, w, dx, dw;
+} zluda_ffn_grouped_grad;
+
+uint32_t zluda_ffn_grouped_backward(const zluda_ffn_grouped_grad *p, void *workspace, size_t workspace_size, void *stream);
+uint32_t zluda_ffn_grouped_backward_workspace(const zluda_ffn_grouped_grad *p, size_t *bytes);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -1,0 +1,112 @@
+"""RMS norm, packing with a scale for each 128, and products of packed operands and grouped by expert (include/zluda_ffn.h, cublasLtMatmul with VEC128_32F
+and BLK128x128_32F) restated in 64 bits, with error bounds for kernels that compute in 32: every value comes with a bound on the error in front of the last
+rounding, as in ffn_oracle.py."""
+import torch
+
+from ffn_oracle import DEPTH, E32, act
+
+BLOCK = 128
+E4M3_HALF, E4M3_LOW = 2.0 ** -4, 2.0 ** -10      # half a step: relative, and at least (of the scale)
+
+
+def blocks(n):
+    return -(-n // BLOCK)
+
+
+def scale_of(v, block_rows=1):
+    """the scales of v (rows x cols, 64 bits): [row block][block], the float nearest to the largest finite magnitude over 448"""
+    rows, cols = v.shape
+    a = torch.where(torch.isfinite(v), v.abs(), torch.zeros_like(v))
+    rb = -(-rows // block_rows)
+    a = torch.nn.functional.pad(a, (0, -cols % BLOCK, 0, rb * block_rows - rows)).reshape(rb, block_rows, -1, BLOCK).amax((1, 3))
+    return (a / 448).float().double().clamp(min=2.0 ** -126)
+
+
+def spread(scales, rows, cols, block_rows=1):
+    return scales.repeat_interleave(block_rows, 0)[:rows].repeat_interleave(BLOCK, 1)[:, :cols]
+
+
+def quantise(q):
+    """q (in units of the scale) on the e4m3 grid, ties to even, and how far it is from the nearest border between two grid values, relative to it"""
+    fin = torch.isfinite(q)
+    z = torch.where(fin, q, torch.zeros_like(q))
+    step = (((torch.frexp(z)[1] - 4).clamp(min=-9).long() + 1023) << 52).view(torch.float64)      # (a power of two, exactly)
+    n = torch.round(z / step)
+    val = n * step
+    off = (step / 2 - (z - val).abs()).abs() / z.abs().clamp(min=2.0 ** -10)
+    return torch.where(fin, val, torch.full_like(val, float("nan"))), off
+
+
+def decode(codes, scales, cols, block_rows=1):
+    """the values that codes (uint8, rows x pitch) and scales [row block][block] stand for, in 64 bits"""
+    c = codes.contiguous().view(torch.float8_e4m3fn).double()[:, :cols]
+    return c * spread(scales.double(), c.shape[0], cols, block_rows)
+
+
+def check_packed(codes, scales, value, bound, cols, block_rows=1, what=""):
+    """codes and scales (as [row block][block]) against the values to be packed and their bounds"""
+    rows = value.shape[0]
+    top = scale_of(value, block_rows)
+    rb = top.shape[0]
+    pad = torch.nn.functional.pad(bound, (0, -cols % BLOCK, 0, rb * block_rows - rows)).reshape(rb, block_rows, -1, BLOCK).amax((1, 3))
+    worst = ((scales.double() - top).abs() / (pad / 448 * 1.01 + 2 * E32 * top)).max().item()
+    assert worst <= 1.0, "%s scales: %.3g times the bound" % (what, worst)
+    got, s = decode(codes, scales, cols, block_rows), spread(scales.double(), rows, cols, block_rows)
+    allowed = torch.maximum(E4M3_HALF * (value.abs() + bound), E4M3_LOW * s) * (1 + 2.0 ** -20) + bound
+    assert torch.isfinite(got).all(), what
+    worst = ((got - value).abs() / allowed).max().item()
+    assert worst <= 1.0, "%s codes: %.3g times the bound" % (what, worst)
+
+
+def rms_forward(h, weight, eps):
+    """from the rounded sum h"""
+    h = h.double()
+    n = h.shape[1]
+    w = torch.ones(n, dtype=torch.float64, device=h.device) if weight is None else weight.double()
+    ms = h.square().mean(1, keepdim=True)
+    rstd = (ms + eps).rsqrt()
+    er = (DEPTH + 6) * E32 / 2 + 5 * E32                         # relative: all terms of the sum are positive
+    y = h * rstd * w
+    return {"y": (y, y.abs() * (er + 3 * E32)), "rstd": (rstd[:, 0], (rstd * er)[:, 0])}
+
+
+def rms_backward(h, dy, weight, rstd, add=None):
+    """from exact h and rstd"""
+    h, dy, rstd = h.double(), dy.double(), rstd.double()[:, None]
+    rows, n = h.shape
+    w = torch.ones(n, dtype=torch.float64, device=h.device) if weight is None else weight.double()
+    xh, v = h * rstd, dy * w
+    m = (v * xh).mean(1, keepdim=True)
+    em = (DEPTH + 6) * E32 * (v * xh).abs().mean(1, keepdim=True)
+    dx = rstd * (v - xh * m)
+    ex = rstd * (xh.abs() * em + 8 * E32 * (v.abs() + (xh * m).abs()))
+    if add is not None:
+        dx, ex = dx + add.double(), ex + 2 * E32 * (dx.abs() + add.double().abs())
+    return {"dx": (dx, ex), "dweight": ((dy * xh).sum(0), (rows + 5) * E32 * (dy * xh).abs().sum(0))}
+
+
+def activated(name, gate, up):
+    """act(gate) * up; name None: a copy"""
+    g = gate.double()
+    if name is None:
+        a, ea = g, torch.zeros_like(g)
+    else:
+        a, _, za, _ = act(name, g)
+        ea = (za + 16) * 4 * E32 * a.abs()
+    if up is None:
+        return a, ea
+    u = up.double()
+    return a * u, ea * u.abs() + 2 * E32 * (a * u).abs()
+
+
+def product(a, b):
+    """a b^T of 64-bit values that are exact, summed in 32 bits in any order, an addition off by a unit in the last place at most"""
+    k = a.shape[1]
+    return a @ b.t(), (k + 4) * 2 * E32 * (a.abs() @ b.abs().t())
+
+
+def scaled_product(a, b, sa, sb):
+    """the same of codes (as values) with scales spread over the elements: two factors and a multiply-add more for each 128 of K"""
+    k = a.shape[1]
+    va, vb = a * sa, b * sb
+    return va @ vb.t(), (k + 4 * blocks(k) + 8) * 2 * E32 * (va.abs() @ vb.abs().t())

@@ -202,7 +202,8 @@ cublasStatus_t desc_attr(MatmulDescObj *o, uint32_t attr, bool set, const void *
       const bool ab = attr == CUBLASLT_MATMUL_DESC_A_SCALE_MODE || attr == CUBLASLT_MATMUL_DESC_B_SCALE_MODE;
       const bool ok = v == CUBLASLT_MATMUL_MATRIX_SCALE_SCALAR_32F ||
                       (ab && (v == CUBLASLT_MATMUL_MATRIX_SCALE_VEC32_UE8M0 ||
-                              v == CUBLASLT_MATMUL_MATRIX_SCALE_OUTER_VEC_32F));
+                              v == CUBLASLT_MATMUL_MATRIX_SCALE_OUTER_VEC_32F || v == CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F ||
+                              v == CUBLASLT_MATMUL_MATRIX_SCALE_BLK128x128_32F));
       if (!ok) return CUBLAS_STATUS_NOT_SUPPORTED;
       m = v;
     }

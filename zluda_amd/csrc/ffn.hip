@@ -2,10 +2,7 @@
 // backward pass are matmuls of the launch layer (include/zluda_gemm_launch.h).
 #include "../../include/zluda_ffn.h"
 
-#include <algorithm>
-#include <cstring>
-
-#include "../../include/zluda_gemm_launch.h"
+#include "ffn_checks.hpp"
 #include "ffn_launchers.hpp"
 #include "kernels/ffn_elementwise.hpp"
 #include "kernels/ffn_norm.hpp"
@@ -19,15 +16,7 @@ namespace {
 // here, with half as much not far enough.  Whole backward passes, us, with 16, 32 and 8 MiB: dX alone, 1001 tokens, 1024 x 2816 30.8, 33.9, 34.9; 500, 4096 x
 // 11008 108, 115, 164; dW alone, 8192, 1024 x 512 37.0, 40.5, 45.5; both, 8192, 1024 x 512 61.9, 64.3, 67.3; 1500, 1023 x 4000 98, 96, 122; 3000, 512 x 512 32.2, 32.2, 29.0.
 constexpr uint64_t kGemmWorkspace = 16ull << 20;
-constexpr int kGridY = 65535;
-
-inline bool is_h16(uint32_t type) { return type == CUDA_R_16F || type == CUDA_R_16BF; }
-inline uint64_t elem_size(uint32_t type) { return type == CUDA_R_32F ? 4 : type == CUDA_R_8F_E4M3 ? 1 : 2; }
 inline uint64_t aligned256(uint64_t n) { return (n + 255) & ~255ull; }
-inline int cus() {
-  const int n = (int)zluda_gemm_device_cu_count();
-  return n ? n : 256;
-}
 
 // a matrix that has to be there: rows x cols of `type`, or a checkpoint where `ckpt` allows one
 uint32_t check_matrix(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, uint32_t type, bool ckpt) {
@@ -42,14 +31,6 @@ uint32_t check_matrix(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, u
   if (m.ld < (int64_t)cols || ((uintptr_t)m.data & (elem_size(type) - 1))) return CUBLAS_STATUS_INVALID_VALUE;
   return CUBLAS_STATUS_SUCCESS;
 }
-#define FFN_CHECK(expr)                            \
-  do {                                             \
-    const uint32_t st_ = (expr);                   \
-    if (st_ != CUBLAS_STATUS_SUCCESS) return st_;  \
-  } while (0)
-
-inline uint32_t check_vector(const void *v, uint32_t type) { return ((uintptr_t)v & (elem_size(type) - 1)) ? CUBLAS_STATUS_INVALID_VALUE : CUBLAS_STATUS_SUCCESS; }
-
 // sizes of a gated layer; tokens may be 0
 uint32_t check_sizes(uint32_t activation, uint64_t tokens, uint64_t features, uint64_t model) {
   if (activation > ZLUDA_FFN_RELU || !features || !model) return CUBLAS_STATUS_INVALID_VALUE;

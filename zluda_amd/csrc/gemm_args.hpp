@@ -12,7 +12,12 @@
 namespace zluda_amd {
 
 enum ScalarMode : int32_t { SCALAR_VALUE = 0, SCALAR_DEV = 1, VECTOR_DEV = 2 };
-enum ScaleMode : int32_t { SCALE_NONE = 0, SCALE_SCALAR = 1, SCALE_OUTER_VEC = 2, SCALE_BLOCK32_UE8M0 = 3 };
+enum ScaleMode : int32_t { SCALE_NONE = 0, SCALE_SCALAR = 1, SCALE_OUTER_VEC = 2, SCALE_BLOCK32_UE8M0 = 3,
+                           SCALE_VEC128 = 4,    // a float for 128 of K of a row: scale[k / 128][row]
+                           SCALE_BLK128 = 5 };  // and of 128 rows: scale[row / 128][k / 128], rows of a multiple of four
+// floats of such scales of one batch
+constexpr int64_t blocks128(int64_t n) { return (n + 127) / 128; }
+constexpr int64_t scales128(int32_t mode, int64_t rows, int64_t k) { return mode == SCALE_VEC128 ? rows * blocks128(k) : blocks128(rows) * ((blocks128(k) + 3) & ~3ll); }
 // (the last two: GELU with its input kept and GELU's gradient where the GEMM kernel does them itself, see aux_mode)
 enum Activation : int32_t { ACT_NONE = 0, ACT_RELU = 1, ACT_GELU = 2, ACT_GELU_KEPT = 3, ACT_DGELU = 4 };
 

@@ -158,7 +158,7 @@ struct ZeroParams {
   void *p;
   int64_t rows, row_bytes, pitch_bytes;  // multiples of 2
 };
-__global__ __launch_bounds__(256) void zero_rows_kernel(ZeroParams z) {
+static __global__ __launch_bounds__(256) void zero_rows_kernel(ZeroParams z) {
   const int64_t words = z.row_bytes / 2;
   for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < z.rows * words; i += (int64_t)gridDim.x * 256)
     ((uint16_t *)((char *)z.p + i / words * z.pitch_bytes))[i % words] = 0;

@@ -9,7 +9,8 @@ namespace zluda_amd {
 constexpr int GEN_T = 64;  // tile edge
 constexpr int GEN_K = 16;  // K per step
 
-template <bool INT_ACC>
+// SC128: a float scale for each 128 of K and row, or 128 rows (SCALE_VEC128, SCALE_BLK128)
+template <bool INT_ACC, bool SC128 = false>
 __global__ __launch_bounds__(256) void gemm_generic_kernel(GemmArgs g) {
   using acc_t = typename std::conditional<INT_ACC, int32_t, float>::type;
   __shared__ acc_t As[GEN_K][GEN_T + 1];
@@ -25,6 +26,10 @@ __global__ __launch_bounds__(256) void gemm_generic_kernel(GemmArgs g) {
   const uint8_t *sb_blk = g.b_scale_mode == SCALE_BLOCK32_UE8M0
                               ? (const uint8_t *)g.b_scale + (int64_t)bt * g.N * KB : nullptr;
 
+  auto scale128 = [](const void *scales, int mode, int rows, int K, int bt, int row, int k) {
+    const float *s = (const float *)scales + bt * scales128(mode, rows, K);
+    return mode == SCALE_VEC128 ? s[(int64_t)(k >> 7) * rows + row] : s[(int64_t)(row >> 7) * ((blocks128(K) + 3) & ~3ll) + (k >> 7)];
+  };
   // thread -> (row, k) of the staging copy; k fastest when the operand is K-contiguous
   const bool a_kfast = g.a_sk == 1, b_kfast = g.b_sk == 1;
 
@@ -50,6 +55,7 @@ __global__ __launch_bounds__(256) void gemm_generic_kernel(GemmArgs g) {
         else {
           float f = load_elem(g.A, g.a_type, idx);
           if (sa_blk) f *= dec_ue8m0(sa_blk[(int64_t)i * KB + (k >> 5)]);
+          if constexpr (SC128) f *= scale128(g.a_scale, g.a_scale_mode, g.M, g.K, bt, i, k);
           v = (acc_t)f;
         }
       }
@@ -65,6 +71,7 @@ __global__ __launch_bounds__(256) void gemm_generic_kernel(GemmArgs g) {
         else {
           float f = load_elem(g.B, g.b_type, idx);
           if (sb_blk) f *= dec_ue8m0(sb_blk[(int64_t)j * KB + (k >> 5)]);
+          if constexpr (SC128) f *= scale128(g.b_scale, g.b_scale_mode, g.N, g.K, bt, j, k);
           v = (acc_t)f;
         }
       }

@@ -422,8 +422,9 @@ uint32_t launch_planned(const zluda_gemm_problem *p, const zluda_gemm_plan *plan
     // (also where a plan for that kernel meets pointers it does not take)
     dim3 grid((l.g.M + 63) / 64, (l.g.N + 63) / 64, l.g.batch);
     const bool int_acc = l.g.a_type == CUDA_R_8I;
-    st = int_acc ? launch_kernel(gemm_generic_kernel<true>, grid, dim3(256), s, l.g)
-                 : launch_kernel(gemm_generic_kernel<false>, grid, dim3(256), s, l.g);
+    st = int_acc                              ? launch_kernel(gemm_generic_kernel<true>, grid, dim3(256), s, l.g)
+         : l.g.a_scale_mode >= SCALE_VEC128 ? launch_kernel(gemm_generic_kernel<false, true>, grid, dim3(256), s, l.g)
+                                            : launch_kernel(gemm_generic_kernel<false>, grid, dim3(256), s, l.g);
     break;
   }
   case ZLUDA_KERNEL_MFMA_I8: case ZLUDA_KERNEL_MFMA_F8: case ZLUDA_KERNEL_MFMA_MXF4: case ZLUDA_KERNEL_MFMA_H16:

@@ -44,6 +44,8 @@ static int convert_scale_mode(int32_t cuda_mode, const void *ptr, bool dry, int3
   case CUBLASLT_MATMUL_MATRIX_SCALE_SCALAR_32F: *out = ptr ? SCALE_SCALAR : SCALE_NONE; return 0;
   case CUBLASLT_MATMUL_MATRIX_SCALE_OUTER_VEC_32F: *out = SCALE_OUTER_VEC; return (ptr || dry) ? 0 : 1;
   case CUBLASLT_MATMUL_MATRIX_SCALE_VEC32_UE8M0: *out = SCALE_BLOCK32_UE8M0; return (ptr || dry) ? 0 : 1;
+  case CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F: *out = SCALE_VEC128; return (ptr || dry) && !((uintptr_t)ptr & 3) ? 0 : 1;
+  case CUBLASLT_MATMUL_MATRIX_SCALE_BLK128x128_32F: *out = SCALE_BLK128; return (ptr || dry) && !((uintptr_t)ptr & 3) ? 0 : 1;
   default: return 2;
   }
 }
@@ -164,6 +166,9 @@ uint32_t lower_problem(const zluda_gemm_problem *p, bool dry, Lowered *out) {
     return CUBLAS_STATUS_INVALID_VALUE;  // cuda_types/src/cublaslt.rs:4266-4267
   if (g.a_scale_mode == SCALE_BLOCK32_UE8M0 && (int_path || g.a_sk != 1 || (K % 32))) return CUBLAS_STATUS_NOT_SUPPORTED;
   if (g.b_scale_mode == SCALE_BLOCK32_UE8M0 && (int_path || g.b_sk != 1 || (K % 32))) return CUBLAS_STATUS_NOT_SUPPORTED;
+  // float scales for 128 of K: 8-bit floats, both operands
+  if ((g.a_scale_mode >= SCALE_VEC128 || g.b_scale_mode >= SCALE_VEC128) &&
+      (int_path || type_bits(a.type) != 8 || g.a_scale_mode < SCALE_VEC128 || g.b_scale_mode < SCALE_VEC128)) return CUBLAS_STATUS_NOT_SUPPORTED;
 
   // ---- epilogue ------------------------------------------------------------------------------
   bool has_bias = false;
@@ -296,7 +301,7 @@ static uint32_t transposing_family(const Lowered &l, bool any_pitch) {
   const bool h16 = g.a_type == CUDA_R_16F || g.a_type == CUDA_R_16BF, f32 = g.a_type == CUDA_R_32F;
   const bool i8 = g.a_type == CUDA_R_8I && g.b_type == CUDA_R_8I;
   const bool f8 = is_f8(g.a_type) && is_f8(g.b_type) && !(g.a_type == CUDA_R_8F_E5M2 && g.b_type == CUDA_R_8F_E5M2);
-  if (!d_type_fast(g) || g.a_scale_mode == SCALE_BLOCK32_UE8M0 || g.b_scale_mode == SCALE_BLOCK32_UE8M0) return 0;
+  if (!d_type_fast(g) || g.a_scale_mode >= SCALE_BLOCK32_UE8M0 || g.b_scale_mode >= SCALE_BLOCK32_UE8M0) return 0;
   if (!(i8 || f8 || ((h16 || f32) && g.b_type == g.a_type))) return 0;
   const int64_t esz = f32 ? 4 : h16 ? 2 : 1;
   const int64_t align = (any_pitch && h16 ? 2 : 4) - 1;
@@ -331,6 +336,7 @@ bool family_supports(uint32_t kernel, const Lowered &l) {
   const GemmArgs &g = l.g;
   const bool fast_layout = l.a_kcontig && l.b_kcontig && l.aligned16;
   const bool d_fast = d_type_fast(g);
+  if (g.a_scale_mode >= SCALE_VEC128) return kernel == ZLUDA_KERNEL_GENERIC;
   switch (kernel) {
   case ZLUDA_KERNEL_GENERIC: return true;
   case ZLUDA_KERNEL_MFMA_I8:
