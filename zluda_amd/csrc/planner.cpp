@@ -78,6 +78,9 @@ uint32_t lower_problem(const zluda_gemm_problem *p, bool dry, Lowered *out) {
   else     { g.b_sj = b_col ? 1 : b.ld; g.b_sk = b_col ? b.ld : 1; }
   g.c_si = c.order == CUBLASLT_ORDER_COL ? 1 : c.ld; g.c_sj = c.order == CUBLASLT_ORDER_COL ? c.ld : 1;
   g.d_si = d.order == CUBLASLT_ORDER_COL ? 1 : d.ld; g.d_sj = d.order == CUBLASLT_ORDER_COL ? d.ld : 1;
+  // a single column with unit stride, of a row-major D of pitch 1: the way to the next one, which nobody goes, lies behind its end, so that what kernels
+  // store past the last column falls outside D as it does elsewhere
+  if (N == 1 && g.d_si == 1) g.d_sj = std::max<int64_t>(g.d_sj, (int64_t)M);
 
   g.batch = d.batch_count;
   if (a.batch_count != g.batch || b.batch_count != g.batch || c.batch_count != g.batch)
@@ -205,6 +208,7 @@ uint32_t lower_problem(const zluda_gemm_problem *p, bool dry, Lowered *out) {
     g.aux = op.epilogue_aux;
     g.aux_si = d.order == CUBLASLT_ORDER_COL ? 1 : op.epilogue_aux_ld;
     g.aux_sj = d.order == CUBLASLT_ORDER_COL ? op.epilogue_aux_ld : 1;
+    if (N == 1 && g.aux_si == 1) g.aux_sj = std::max<int64_t>(g.aux_sj, (int64_t)M);
     g.aux_sb = op.epilogue_aux_batch_stride;
     if (g.aux_bgrad) {
       if (g.batch > 1 && op.bias_batch_stride == 0) return CUBLAS_STATUS_NOT_SUPPORTED;
