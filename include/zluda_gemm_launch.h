@@ -84,7 +84,8 @@ enum {
   ZLUDA_KERNEL_MFMA_H16 = 7,  /* v_mfma_f32_32x32x16_f16 / _bf16, K-contiguous A and B of one 16-bit type */
   ZLUDA_KERNEL_MFMA_TR16 = 8, /* f16 / bf16 MFMA with transposing loads: A or B not K-contiguous */
   ZLUDA_KERNEL_MFMA_F32 = 9,  /* v_mfma_f32_32x32x2_f32, K-contiguous f32 A and B */
-  ZLUDA_KERNEL_MFMA_TR32 = 10 /* f32 MFMA with transposing loads: A or B not K-contiguous */
+  ZLUDA_KERNEL_MFMA_TR32 = 10, /* f32 MFMA with transposing loads: A or B not K-contiguous */
+  ZLUDA_KERNEL_MFMA_BLK8 = 11 /* v_mfma_f32_16x16x128_f8f6f4, K-contiguous fp8 with a float scale for each 128 of K */
 };
 
 /* The 64-byte algo blob the application round-trips between the heuristic and cublasLtMatmul

@@ -76,7 +76,7 @@ def run(api, m, n, k, a_mode=BLK, b_mode=VEC, a="e4m3", b="e4m3", out="bf16", ac
     what = "%dx%dx%d kernel %d/%d" % (m, n, k, got_kernel, got_variant)
     assert D.guards(), what
     for i in range(batch):
-        v, e = P.scaled_product(B.codes[i], A.codes[i], B.spread[i], A.spread[i])      # n x m
+        v, e = P.scaled_product(B.codes[i], A.codes[i], B.spread[i], A.spread[i], out == "f32")      # n x m
         v, e = v * alpha, e * abs(alpha) + 2 * O.E32 * abs(alpha) * v.abs()
         if row_major:
             v, e = v.t(), e.t()
@@ -90,7 +90,8 @@ def run(api, m, n, k, a_mode=BLK, b_mode=VEC, a="e4m3", b="e4m3", out="bf16", ac
             v = v.clamp(min=0)
         elif act == "gelu":
             a_, _, za, _ = O.act("gelu", v)
-            v, e = a_, 1.13 * e + (za + 16) * 4 * O.E32 * a_.abs()
+            # (the sigmoid comes out of v_rcp_f32, whose results below 2^-126, the smallest normal number, are zeros: up to |v| 2^-126)
+            v, e = a_, 1.13 * e + (za + 16) * 4 * O.E32 * a_.abs() + (v.abs() + e) * 2.0 ** -126
         if d_scale is not None:
             v, e = v * d_scale, e * abs(d_scale) + O.E32 * (v * d_scale).abs()
         O.check(D.view[i * q:(i + 1) * q], (v, e), what)
@@ -104,6 +105,20 @@ def test_sizes(gpu_api, m, n, k):
         run(gpu_api, m, n, k, a_mode, b_mode)
     run(gpu_api, m, n, k, workspace=0)
     run(gpu_api, m, n, k, VEC, BLK, row_major=True)
+
+
+@pytest.mark.parametrize("variant", [0, 1, 2, 3])
+@pytest.mark.parametrize("k", [16, 128, 256, 272, 384, 512, 640, 784, 1040, 1152, 2048])
+def test_every_tile_at_every_length(gpu_api, variant, k):
+    """counts of stages around those of the rings, whole tiles and ragged ones, shared out along K and not"""
+    for m, n in ((256, 256), (130, 40), (300, 290), (520, 1)):
+        for modes in ((BLK, VEC), (BLK, BLK), (VEC, VEC), (VEC, BLK)):
+            if variant == 0 and modes[0] == VEC:
+                continue
+            assert run(gpu_api, m, n, k, *modes, kernel=K.ZLUDA_KERNEL_MFMA_BLK8, variant=variant) == (K.ZLUDA_KERNEL_MFMA_BLK8, variant)
+            if variant >= 2:
+                assert run(gpu_api, m, n, k, *modes, out="f32", kernel=K.ZLUDA_KERNEL_MFMA_BLK8, variant=variant) == (K.ZLUDA_KERNEL_MFMA_BLK8, variant)
+        run(gpu_api, m, n, k, BLK, VEC, kernel=K.ZLUDA_KERNEL_MFMA_BLK8, variant=variant, workspace=0, act="gelu", bias=1, pad=16)
 
 
 @pytest.mark.parametrize("a,b", [("e4m3", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e4m3"), ("e5m2", "e5m2")])

@@ -312,7 +312,7 @@ bool unpack_algo(const cublasLtMatmulAlgo_t *algo, uint32_t *kernel, int32_t *va
   if ((algo->data[0] >> 32) != ZLUDA_ALGO_MAGIC) return false;
   *kernel = (uint32_t)(algo->data[0] & 0xffffffffu);
   *variant = (int32_t)algo->data[1];
-  return *kernel >= ZLUDA_KERNEL_GENERIC && *kernel <= ZLUDA_KERNEL_MFMA_TR32;
+  return *kernel >= ZLUDA_KERNEL_GENERIC && *kernel <= ZLUDA_KERNEL_MFMA_BLK8;
 }
 
 // A/B forcing for measurements: ZLUDA_FORCE_KERNEL=<family>[:<variant>], read once per process (the

@@ -146,6 +146,34 @@ uint32_t launch_mfma(const Lowered &l, const zluda_gemm_plan &plan_in, void *ws,
   return launch_splitk_reduce(rp, np, nq, s);
 }
 
+// products with a scale for each 128 of K
+uint32_t launch_block(const Lowered &l, const zluda_gemm_plan &plan, void *ws, uint64_t ws_size, hipStream_t s) {
+  if (plan.variant >= (uint32_t)kNumBlockVariants) return CUBLAS_STATUS_INVALID_VALUE;
+  const BlockVariant &v = kBlockVariants[plan.variant];
+  MfmaParams prm;
+  prm.g = l.g;
+  prm.swapped = plan.swapped;
+  const int np = plan.swapped ? l.g.N : l.g.M, nq = plan.swapped ? l.g.M : l.g.N;
+  prm.tiles_p = (np + v.bp - 1) / v.bp;
+  prm.tiles_q = (nq + v.bq - 1) / v.bq;
+  prm.group_p = 8;
+  prm.splits = 1; prm.split_stages = 0; prm.groups = 0; prm.ws = nullptr;
+  if (plan.swapped != (uint32_t)(l.g.d_si != 1) || (uint32_t)(prm.tiles_p * prm.tiles_q) != plan.grid_x || (uint32_t)l.g.batch != plan.grid_y) return CUBLAS_STATUS_INVALID_VALUE;
+  if (plan.grid_z > 1) {
+    const uint64_t need = (uint64_t)plan.grid_z * l.g.batch * prm.tiles_p * v.bp * prm.tiles_q * v.bq * 4;
+    if (!ws || (((uintptr_t)ws) & 15) || ws_size < need || plan.workspace < need) return CUBLAS_STATUS_INVALID_VALUE;
+    prm.splits = (int32_t)plan.grid_z;
+    prm.split_stages = (int32_t)((blocks128(l.g.K) + prm.splits - 1) / prm.splits);
+    prm.ws = ws;
+  }
+  const uint32_t fp = f8_fmt(plan.swapped ? l.g.b_type : l.g.a_type), fq = f8_fmt(plan.swapped ? l.g.a_type : l.g.b_type);
+  const bool uniform = block_uniform_p(l), exact = block_exact(l);
+  const uint32_t st = (fp ? launch_block_f8_e5m2p : fq ? launch_block_f8_e5m2q : launch_block_f8_e4m3)(prm, plan, uniform, exact, s);
+  if (st || prm.splits == 1) return st;
+  const SplitKReduceParams rp{l.g, (int32_t)plan.swapped, prm.splits, 0, prm.tiles_p * v.bp, prm.tiles_q * v.bq, (const int32_t *)ws};
+  return launch_splitk_reduce(rp, np, nq, s);
+}
+
 uint32_t launch_tr(const Lowered &l, const zluda_gemm_plan &plan, void *ws, uint64_t ws_size, hipStream_t s) {
   if (plan.variant >= (uint32_t)kNumTrVariants) return CUBLAS_STATUS_INVALID_VALUE;
   const TrVariant &v = kTrVariants[plan.variant];
@@ -432,6 +460,7 @@ uint32_t launch_planned(const zluda_gemm_problem *p, const zluda_gemm_plan *plan
     st = launch_mfma(l, *plan, ws, ws_size, s);
     break;
   case ZLUDA_KERNEL_DECODE_W8A8: st = launch_decode(l, *plan, s); break;
+  case ZLUDA_KERNEL_MFMA_BLK8: st = launch_block(l, *plan, ws, ws_size, s); break;
   case ZLUDA_KERNEL_MFMA_TR8: case ZLUDA_KERNEL_MFMA_TR16: case ZLUDA_KERNEL_MFMA_TR32: st = launch_tr(l, *plan, ws, ws_size, s); break;
   default: return CUBLAS_STATUS_NOT_SUPPORTED;
   }

@@ -70,6 +70,10 @@ uint32_t launch_mfma_h16(const MfmaParams &prm, const zluda_gemm_plan &plan, boo
 uint32_t launch_mfma_aux_f16(const MfmaParams &prm, const zluda_gemm_plan &plan, hipStream_t s);
 uint32_t launch_mfma_aux_bf16(const MfmaParams &prm, const zluda_gemm_plan &plan, hipStream_t s);
 uint32_t launch_mfma_f32(const MfmaParams &prm, const zluda_gemm_plan &plan, hipStream_t s);
+// a scale for each 128 of K (block_launch.hpp); formats of P and Q: both E4M3, Q E5M2, P E5M2
+uint32_t launch_block_f8_e4m3(const MfmaParams &prm, const zluda_gemm_plan &plan, bool uniform, bool exact, hipStream_t s);
+uint32_t launch_block_f8_e5m2q(const MfmaParams &prm, const zluda_gemm_plan &plan, bool uniform, bool exact, hipStream_t s);
+uint32_t launch_block_f8_e5m2p(const MfmaParams &prm, const zluda_gemm_plan &plan, bool uniform, bool exact, hipStream_t s);
 // variant 3 in the form of kernels/gemm_mfma_short.hpp; `grid` workgroups, prm.groups the same number
 uint32_t launch_mfma_short(const MfmaParams &prm, bool bf16, uint32_t grid, hipStream_t s);
 // the four-wave persistent kernel (variant 11; kernels/gemm_mfma_w4.hpp), `epi` = W4_CLASS_* of planner.hpp, `grid` workgroups

@@ -340,7 +340,13 @@ bool family_supports(uint32_t kernel, const Lowered &l) {
   const GemmArgs &g = l.g;
   const bool fast_layout = l.a_kcontig && l.b_kcontig && l.aligned16;
   const bool d_fast = d_type_fast(g);
-  if (g.a_scale_mode >= SCALE_VEC128) return kernel == ZLUDA_KERNEL_GENERIC;
+  if (g.a_scale_mode >= SCALE_VEC128) {
+    if (kernel == ZLUDA_KERNEL_GENERIC) return true;
+    // (a tile reaches its rows and its scales through windows of 2 GiB)
+    auto in_window = [&](int64_t ld, int64_t rows) { return ld < (1 << 22) && rows * blocks128(g.K) < (1 << 28); };
+    return kernel == ZLUDA_KERNEL_MFMA_BLK8 && fast_layout && d_fast && !(g.a_type == CUDA_R_8F_E5M2 && g.b_type == CUDA_R_8F_E5M2) &&
+           in_window(g.a_si, g.M) && in_window(g.b_sj, g.N);
+  }
   switch (kernel) {
   case ZLUDA_KERNEL_GENERIC: return true;
   case ZLUDA_KERNEL_MFMA_I8:
@@ -814,6 +820,42 @@ uint32_t aux_sum_shares(const Lowered &l, const zluda_gemm_plan &plan) {
   return ceil_div(l.g.N, kTrVariants[plan.variant].bq) * kTrVariants[plan.variant].wq;
 }
 
+bool block_uniform_p(const Lowered &l) { return (l.g.d_si != 1 ? l.g.b_scale_mode : l.g.a_scale_mode) == SCALE_BLK128; }
+
+bool block_exact(const Lowered &l) { return l.g.d_type == CUDA_R_32F; }
+
+static void fill_block_plan(const Lowered &l, int variant, uint32_t cus, uint64_t workspace_size, zluda_gemm_plan *plan) {
+  const GemmArgs &g = l.g;
+  const BlockVariant &v = kBlockVariants[variant];
+  const uint32_t np = g.d_si != 1 ? g.N : g.M, nq = g.d_si != 1 ? g.M : g.N;
+  plan->variant = variant;
+  plan->swapped = g.d_si != 1;
+  plan->grid_x = ceil_div(np, v.bp) * ceil_div(nq, v.bq); plan->grid_y = g.batch; plan->grid_z = 1;
+  plan->block = v.wp * v.wq * 64;
+  plan->workspace = 0;
+  const uint64_t tiles = (uint64_t)plan->grid_x * plan->grid_y, stages = (uint64_t)blocks128(g.K);
+  if (tiles * 2 <= cus && stages >= 8) {
+    uint64_t s = std::min<uint64_t>({8, cus / tiles, stages / 4});
+    const uint64_t each = (uint64_t)g.batch * ceil_div(np, v.bp) * v.bp * ceil_div(nq, v.bq) * v.bq * 4;
+    while (s > 1 && s * each > workspace_size) s--;
+    if (s > 1) {
+      plan->grid_z = (uint32_t)s;
+      plan->workspace = s * each;
+    }
+  }
+  plan->waves = (float)(tiles * plan->grid_z) / (float)cus;
+}
+
+static int pick_block_variant(const Lowered &l, uint32_t cus, uint64_t workspace_size) {
+  const GemmArgs &g = l.g;
+  const uint32_t np = g.d_si != 1 ? g.N : g.M, nq = g.d_si != 1 ? g.M : g.N;
+  auto tiles = [&](int v) { return (uint64_t)ceil_div(np, kBlockVariants[v].bp) * ceil_div(nq, kBlockVariants[v].bq) * g.batch; };
+  if (nq <= 32) return 3;
+  if (block_exact(l)) return 2;
+  if (block_uniform_p(l) && tiles(0) >= cus) return 0;
+  return tiles(1) >= cus ? 1 : 2;
+}
+
 uint32_t transposing_under_generic(const Lowered &l) {
   const uint32_t family = transposing_family(l, true);
   if (!family || transposing_family(l, false)) return 0;
@@ -916,6 +958,7 @@ extern "C" uint32_t zluda_gemm_variant_count(uint32_t kernel) {
   case ZLUDA_KERNEL_DECODE_W8A8: return kNumDecodeVariants;
   case ZLUDA_KERNEL_MFMA_TR8: case ZLUDA_KERNEL_MFMA_TR16: return kNumTrVariants;
   case ZLUDA_KERNEL_MFMA_TR32: return kNumTrVariants - 1;  // the 16x16-shape one is not instantiated for f32
+  case ZLUDA_KERNEL_MFMA_BLK8: return kNumBlockVariants;
   default: return 0;
   }
 }
@@ -934,7 +977,7 @@ extern "C" uint32_t zluda_gemm_plan_problem(const zluda_gemm_problem *p, uint32_
   if (kernel == ZLUDA_KERNEL_AUTO) {
     static const uint32_t order[] = {ZLUDA_KERNEL_DECODE_W8A8, ZLUDA_KERNEL_MFMA_I8, ZLUDA_KERNEL_MFMA_F8,
                                      ZLUDA_KERNEL_MFMA_MXF4, ZLUDA_KERNEL_MFMA_H16, ZLUDA_KERNEL_MFMA_TR8,
-                                     ZLUDA_KERNEL_MFMA_TR16, ZLUDA_KERNEL_MFMA_F32, ZLUDA_KERNEL_MFMA_TR32, ZLUDA_KERNEL_GENERIC};
+                                     ZLUDA_KERNEL_MFMA_TR16, ZLUDA_KERNEL_MFMA_F32, ZLUDA_KERNEL_MFMA_TR32, ZLUDA_KERNEL_MFMA_BLK8, ZLUDA_KERNEL_GENERIC};
     for (uint32_t k : order) {
       if (!family_supports(k, l)) continue;
       if (k == ZLUDA_KERNEL_DECODE_W8A8) {
@@ -1002,6 +1045,13 @@ extern "C" uint32_t zluda_gemm_plan_problem(const zluda_gemm_problem *p, uint32_
     if (v >= kNumTrVariants || (kTrVariants[v].m16 && l.g.a_type != CUDA_R_8I && l.g.a_type != CUDA_R_16F && l.g.a_type != CUDA_R_16BF))
       return CUBLAS_STATUS_INVALID_VALUE;
     fill_tr_plan(l, v, cu_count, p->workspace_size, plan);
+    break;
+  }
+  case ZLUDA_KERNEL_MFMA_BLK8: {
+    const int v = forced_variant >= 0 ? forced_variant : pick_block_variant(l, cu_count, p->workspace_size);
+    if (v >= kNumBlockVariants) return CUBLAS_STATUS_INVALID_VALUE;
+    if ((kBlockVariants[v].uniform && !block_uniform_p(l)) || (!kBlockVariants[v].exact && block_exact(l))) return CUBLAS_STATUS_NOT_SUPPORTED;
+    fill_block_plan(l, v, cu_count, p->workspace_size, plan);
     break;
   }
   case ZLUDA_KERNEL_DECODE_W8A8: {

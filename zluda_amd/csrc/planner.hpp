@@ -51,6 +51,17 @@ constexpr int kTr64Stages[] = {6, 3, 2};  // and of variant 2: up to one workgro
 constexpr int tr_ring_stages(int variant, uint64_t groups, uint64_t cus) {
   return variant == 1 ? (groups <= cus ? kTrDeepStages : 2) : variant == 2 ? kTr64Stages[groups <= cus ? 0 : groups <= 3 * cus ? 1 : 2] : 2;
 }
+// tile configurations of the products with a scale for each 128 of K (index = plan.variant for ZLUDA_KERNEL_MFMA_BLK8): workgroup tile, waves, LDS
+// stages of 128 K bytes; uniform: only for P rows that share their scales (the accumulators of a wave leave no registers for more); exact: also for results in
+// 32 bits (the widened operands take registers)
+struct BlockVariant { int bp, bq, wp, wq, stages; bool uniform, exact; };
+constexpr BlockVariant kBlockVariants[] = {
+    {256, 256, 2, 4, 2, true, false},   // 0
+    {128, 128, 2, 2, 2, false, false},  // 1: two workgroups per CU
+    {64, 64, 2, 2, 4, false, true},     // 2: two
+    {64, 32, 2, 2, 4, false, true},     // 3: three
+};
+constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
 constexpr int kNumTrVariants = sizeof(kTrVariants) / sizeof(kTrVariants[0]);
 
 // decode configurations (index = plan.variant for ZLUDA_KERNEL_DECODE_W8A8).
@@ -111,6 +122,11 @@ struct Lowered {
 // Validates `p` and fills `out`.  With dry=true (heuristic time) data pointers and host scalars are
 // not dereferenced and NULL data pointers are allowed.
 uint32_t lower_problem(const zluda_gemm_problem *p, bool dry, Lowered *out);
+
+// whether the rows of the operand that runs along D's unit stride share their scales for 128 of K in blocks of 128
+bool block_uniform_p(const Lowered &l);
+// whether its products keep 32 bits, for a D that does
+bool block_exact(const Lowered &l);
 
 // the fast epilogue of the four-wave kernel that serves the problem, or W4_CLASS_NONE; `dry`: planning (beta and the
 // pointers are not known yet and are taken to be zero / aligned)
