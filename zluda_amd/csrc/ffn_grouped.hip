@@ -2,7 +2,7 @@
 #include "../../include/zluda_ffn.h"
 
 #include "ffn_checks.hpp"
-#include "kernels/ffn_grouped.hpp"
+#include "ffn_grouped_launch.hpp"
 
 using namespace zluda_amd;
 
@@ -56,6 +56,44 @@ dim3 any_grid(uint64_t cols, uint64_t rows, uint64_t experts) {
   return dim3((uint32_t)((cols + 63) / 64), (uint32_t)std::min<uint64_t>((rows + 63) / 64 + std::min(experts, rows), kGridY));
 }
 
+// 16-byte pieces of the operands' rows; tiles whose rows, and the scales of a block of K, lie within reach of 32-bit offsets
+bool tile_operands(const zluda_ffn_grouped *p) {
+  const int64_t size = (int64_t)elem_size(p->x.type);
+  const bool aligned = !(((uintptr_t)p->x.data | (uintptr_t)p->w.data | (uintptr_t)(p->x.ld * size) | (uintptr_t)(p->w.ld * size) | (p->model * size)) & 15);
+  const bool near = p->x.ld < kNarrowPitch && p->w.ld < kNarrowPitch && p->y.ld < kNarrowPitch &&
+                    (size != 1 || (p->x.ld_scales * (int64_t)((p->model + 127) / 128) < (1 << 28) && p->w.ld_scales < (1 << 28)));
+  return aligned && near;
+}
+
+// The tile whose last workgroup is done first, if the rows are shared out about evenly, which only the device knows: a tile for each expert, and beyond that half
+// of one that is not full for each.  Measured, us, in the order of kBlockTiles: 2048 of model, 5632 features, eight experts, bf16, 16 rows 56, 42, 37, 35; 256 61,
+// 45, 39, 42; 512 62, 48, 50, 54; 2048 96, 82, 105, 126; 4096 117, 138, 172, 219; 1024 of model, 2816 features, 64 experts, 1024 rows 91, 77, 76, 71; 4096 106, 91, 97, 105.
+int pick_tile(const zluda_ffn_grouped *p) {
+  const bool eight = p->x.type == CUDA_R_8F_E4M3, exact = eight && p->y.type == CUDA_R_32F;
+  const uint64_t live = std::min(p->rows, p->experts), stages = (p->model * (eight ? 1 : 2) + 127) / 128;
+  int best = -1;
+  float best_us = 0.0f;
+  for (int v = exact ? 2 : 0; v < kBlockTileCount; v++) {
+    const uint64_t q = std::max<uint64_t>(live, p->rows / kBlockTiles[v].bq + (live + 1) / 2);
+    const float us = block_tiles_us(v, q * ((p->features + kBlockTiles[v].bp - 1) / kBlockTiles[v].bp), stages, (uint64_t)cus(), eight);
+    if (best < 0 || us < best_us) {
+      best = v;
+      best_us = us;
+    }
+  }
+  return best;
+}
+
+// the same for the gradients, through windows of 2 GiB on an expert's matrices and rows; whole pieces of eight along every row
+bool tile_operands(const zluda_ffn_grouped_grad *p) {
+  uintptr_t at = (uintptr_t)p->dy.data;
+  int64_t ld = p->dy.ld, most = p->dy.ld;
+  if (p->dx.data) { at |= (uintptr_t)p->w.data | (uintptr_t)p->dx.data; ld |= p->w.ld | p->dx.ld; most = std::max({most, p->w.ld, p->dx.ld}); }
+  if (p->dw.data) { at |= (uintptr_t)p->x.data | (uintptr_t)p->dw.data; ld |= p->x.ld | p->dw.ld; most = std::max({most, p->x.ld, p->dw.ld}); }
+  if ((at & 15) || (ld & 7) || (p->model & 7) || (p->features & 7) || most >= kNarrowPitch) return false;
+  return in_window(p->rows, p->dy.ld) && (!p->dx.data || in_window(p->features, p->w.ld)) && (!p->dw.data || in_window(p->rows, p->x.ld));
+}
+
 } // namespace
 
 extern "C" uint32_t zluda_ffn_grouped_forward_workspace(const zluda_ffn_grouped *p, size_t *bytes) {
@@ -70,6 +108,11 @@ extern "C" uint32_t zluda_ffn_grouped_forward(const zluda_ffn_grouped *p, void *
   if (!zluda_gemm_device_cu_count()) return CUBLAS_STATUS_NOT_INITIALIZED;
   const GroupedParams g{p->offsets, p->x.data, p->w.data, p->y.data, (const float *)p->x.scales, (const float *)p->w.scales, p->x.ld, p->w.ld, p->y.ld,
                         p->x.ld_scales, p->w.ld_scales, (int32_t)p->rows, (int32_t)p->experts, (int32_t)p->features, (int32_t)p->model, p->x.type, p->y.type};
+  if (tile_operands(p)) {
+    const int tile = pick_tile(p);
+    if (((p->features + kBlockTiles[tile].bp - 1) / kBlockTiles[tile].bp) * most_row_tiles(p->rows, p->experts, kBlockTiles[tile].bq) < (1ull << 31))
+      return (p->x.type == CUDA_R_16BF ? launch_grouped_bf16 : p->x.type == CUDA_R_16F ? launch_grouped_f16 : launch_grouped_f8)(g, tile, (hipStream_t)stream);
+  }
   return launch_kernel(grouped_any_kernel<0>, any_grid(p->features, p->rows, p->experts), dim3(256), (hipStream_t)stream, g);
 }
 
@@ -83,6 +126,17 @@ extern "C" uint32_t zluda_ffn_grouped_backward(const zluda_ffn_grouped_grad *p, 
   FFN_CHECK(check_backward(p));
   if (!zluda_gemm_device_cu_count()) return CUBLAS_STATUS_NOT_INITIALIZED;
   const hipStream_t s = (hipStream_t)stream;
+  if (tile_operands(p)) {
+    auto tiles = [](uint64_t n) { return (n + kGradTile - 1) / kGradTile; };
+    const uint64_t dx = p->dx.data && p->rows ? tiles(p->model) * most_row_tiles(p->rows, p->experts, kGradTile) : 0;
+    const uint64_t dw = p->dw.data ? tiles(p->model) * tiles(p->features) * p->experts : 0;
+    if (dx + dw == 0) return CUBLAS_STATUS_SUCCESS;
+    if (dx + dw < (1ull << 31)) {
+      const GroupedGradParams q{p->offsets, p->dy.data, p->x.data, p->w.data, p->dx.data, p->dw.data, p->dx.ld, p->dw.ld, (int32_t)p->dy.ld, (int32_t)p->x.ld, (int32_t)p->w.ld,
+                                (int32_t)p->rows, (int32_t)p->experts, (int32_t)p->features, (int32_t)p->model, (uint32_t)dx};
+      return launch_grouped_grad(q, p->dy.type, (uint32_t)(dx + dw), s);
+    }
+  }
   GroupedParams g{p->offsets, p->dy.data, p->w.data, p->dx.data, nullptr, nullptr, p->dy.ld, p->w.ld, p->dx.ld, 0, 0, (int32_t)p->rows, (int32_t)p->experts,
                   (int32_t)p->features, (int32_t)p->model, p->dy.type, p->dy.type};
   if (p->dx.data && p->rows) FFN_CHECK(launch_kernel(grouped_any_kernel<1>, any_grid(p->model, p->rows, p->experts), dim3(256), s, g));

@@ -83,7 +83,9 @@ struct RingTile {
   static constexpr int SP = BP < 64 ? 64 : BP, SQ = BQ < 64 ? 64 : BQ, PIECES = (SP + SQ) / 64, LS = F8 ? (PIECES + NW - 1) / NW : 0;
   static constexpr int NLOAD = LP + LQ + LS;
   static constexpr int TP = BP / WP / 16, TQ = BQ / WQ / 16;
-  static constexpr int SLOT = (BP + BQ) * 8 + (F8 ? (SP + SQ) / 4 : 0), WORDS = NS * SLOT;  // 16-byte words
+  // 16-byte words: the slots, behind them the scales of one stage more than there are slots (those of P's rows are read while their stage is multiplied, when its
+  // slot is already being refilled)
+  static constexpr int SLOT = (BP + BQ) * 8, S_SLOT = F8 ? (SP + SQ) / 4 : 0, S_AT = NS * SLOT, WORDS = S_AT + (NS + 1) * S_SLOT;
   static_assert(RPP % 32 == 0 && BP % RPP == 0 && BQ % RPP == 0 && (BP / WP) % 32 == 0 && BQ % (16 * WQ) == 0, "whole passes, whole pairs of tiles");
   static_assert(WORDS * 16 <= 160 * 1024 && (NS - 1) * NLOAD < 64 && NS >= 2, "LDS and vmcnt");
 
@@ -116,7 +118,7 @@ struct RingTile {
       const int row = min((piece < SP / 64 ? piece : piece - SP / 64) * 64 + lane, min(piece < SP / 64 ? BP : BQ, side.rows) - 1);
       os[i] = (side.per_row ? row * side.s_row : (row >> 7) * side.s_row) * 4;
     }
-    auto issue = [&](auto i_c, int kt, int slot) __attribute__((always_inline)) {  // instruction i of a stage
+    auto issue = [&](auto i_c, int kt, int slot, int s_slot) __attribute__((always_inline)) {  // instruction i of a stage
       constexpr int i = decltype(i_c)::value;
       const int st = first + (kt + turn < stages ? kt + turn : kt + turn - stages), at = st * 128;
       v4i *base = &lds[slot * SLOT];
@@ -127,24 +129,25 @@ struct RingTile {
       } else {
         constexpr int j = i - LP - LQ;
         const int piece = (wave + NW * j) % PIECES;
-        float *to = (float *)(base + (BP + BQ) * 8) + piece * 64;
+        float *to = (float *)&lds[S_AT + s_slot * S_SLOT] + piece * 64;
         if (piece < SP / 64) lds_dma4(rsp, to, os[j], st * P.s_step * 4);  // (uniform)
         else lds_dma4(rsq, to, os[j], st * Q.s_step * 4);
       }
     };
 
     // ---- fragments ----------------------------------------------------------------------------------------------------------------
-    constexpr int NF = 2 * (TP + TQ), NSC = F8 ? (SU ? 1 : TP) + TQ : 0, NR = NF + NSC, NM = TP * TQ * kBlockSteps<KIND>;  // LDS reads and MFMAs of a stage
+    constexpr int NF = 2 * (TP + TQ), NSC = F8 ? TQ + (SU ? 1 : 0) : 0, NR = NF + NSC, NM = TP * TQ * kBlockSteps<KIND>;  // LDS reads and MFMAs of a stage
     v4i fr[2][TP + TQ][2];                      // [stage parity][P tiles, Q tiles][half of a lane's 32 bytes]
-    v4f sp[2][F8 && !SU ? TP : 1];              // scales: of a lane's four rows of each P tile, or one
-    float sq[2][F8 ? TQ : 1];                   // and of its column of each Q tile
+    float sp[2];                                // scales: the one of the wave's P rows
+    float sq[2][F8 ? TQ : 1];                   // and of a lane's column of each Q tile
+    v4f sr[2];                                  // of its four rows of a P tile, and of the next
     int at_p[2], at_q[2];                       // [half]
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       at_p[h] = (wp * (16 * TP) + r16) * 8 + ((2 * grp + h) ^ swz_block(r16));
       at_q[h] = (BP + wq * (16 * TQ) + r16) * 8 + ((2 * grp + h) ^ swz_block(r16));
     }
-    auto read = [&](auto r_c, auto cur_c, int slot) __attribute__((always_inline)) {  // LDS read r of a stage
+    auto read = [&](auto r_c, auto cur_c, int slot, int s_slot) __attribute__((always_inline)) {  // LDS read r of a stage
       constexpr int r = decltype(r_c)::value, cur = decltype(cur_c)::value;
       const v4i *base = &lds[slot * SLOT];
       if constexpr (r < NF) {
@@ -152,10 +155,9 @@ struct RingTile {
         fr[cur][i][h] = base[(i < TP ? at_p : at_q)[h] + tile * 128];
       } else {
         constexpr int j = r - NF;
-        const float *s = (const float *)(base + (BP + BQ) * 8);
+        const float *s = (const float *)&lds[S_AT + s_slot * S_SLOT];
         if constexpr (j < TQ) sq[cur][j] = s[SP + wq * (16 * TQ) + 16 * j + r16];
-        else if constexpr (SU) sp[cur][0][0] = s[wp * (16 * TP)];
-        else sp[cur][j - TQ] = *(const v4f *)(s + wp * (16 * TP) + 16 * (j - TQ) + 4 * grp);
+        else sp[cur] = s[wp * (16 * TP)];
       }
     };
     // waits until at most `younger` stages of this wave's instructions are outstanding
@@ -166,23 +168,23 @@ struct RingTile {
       });
     };
     static_for<NS>([&](auto st_c) {
-      if (decltype(st_c)::value < stages) static_for<NLOAD>([&](auto i_c) { issue(i_c, decltype(st_c)::value, decltype(st_c)::value); });
+      if (decltype(st_c)::value < stages) static_for<NLOAD>([&](auto i_c) { issue(i_c, decltype(st_c)::value, decltype(st_c)::value, decltype(st_c)::value); });
     });
     wait_for(min(stages, NS) - 1);
-    static_for<NR>([&](auto r_c) { read(r_c, std::integral_constant<int, 0>{}, 0); });
-    int slot = 0;
+    static_for<NR>([&](auto r_c) { read(r_c, std::integral_constant<int, 0>{}, 0, 0); });
+    int slot = 0, s_slot = 0;
     auto do_stage = [&](auto cur_c, auto refill_c, int kt) __attribute__((always_inline)) {
       constexpr int cur = decltype(cur_c)::value;
       constexpr bool REFILL = decltype(refill_c)::value != 0;  // stage kt + NS exists
       using Next = std::integral_constant<int, 1 - cur>;
-      const int next = slot == NS - 1 ? 0 : slot + 1;
+      const int next = slot == NS - 1 ? 0 : slot + 1, s_next = s_slot == NS ? 0 : s_slot + 1, s_last = s_slot == 0 ? NS : s_slot - 1;  // (stage kt + NS's)
       if constexpr (REFILL) wait_vmcnt_barrier<(NS - 2) * NLOAD>();
       else wait_for(min(stages - kt, NS) - 2);
       __builtin_amdgcn_sched_barrier(0);
       float s[F8 ? TQ : 1];
       if constexpr (F8 && SU) {
 #pragma unroll
-        for (int b = 0; b < TQ; b++) s[b] = sp[cur][0][0] * sq[cur][b];
+        for (int b = 0; b < TQ; b++) s[b] = sp[cur] * sq[cur][b];
       }
       v8b wide[EXACT ? TP + TQ : 1][4];
       if constexpr (EXACT) {
@@ -191,13 +193,15 @@ struct RingTile {
           block_widen<i < TP ? FP : FQ>(fr[cur][i], wide[i]);
         });
       }
+      const float *const rows = (const float *)&lds[S_AT + s_slot * S_SLOT] + wp * (16 * TP) + 4 * grp;
+      if constexpr (F8 && !SU) sr[0] = *(const v4f *)rows;
       v4f t[3];
       auto add = [&](auto x_c) __attribute__((always_inline)) {
         constexpr int x = decltype(x_c)::value, a = x / TQ, b = x % TQ;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           if constexpr (SU) acc[a][b][e] = __builtin_fmaf(t[x % 3][e], s[b], acc[a][b][e]);
-          else acc[a][b][e] = __builtin_fmaf(t[x % 3][e], sp[cur][F8 && !SU ? a : 0][e] * sq[cur][F8 ? b : 0], acc[a][b][e]);
+          else acc[a][b][e] = __builtin_fmaf(t[x % 3][e], sr[a & 1][e] * sq[cur][F8 ? b : 0], acc[a][b][e]);
         }
       };
       static_for<NM>([&](auto x_c) {
@@ -211,15 +215,19 @@ struct RingTile {
         } else if constexpr (F8) t[x % 3] = block_mfma<KIND, FP, FQ>(fr[cur][a], fr[cur][TP + b], 0, v4f{0.0f, 0.0f, 0.0f, 0.0f});
         else acc[a][b] = block_mfma<KIND, FP, FQ>(fr[cur][a], fr[cur][TP + b], x / (TP * TQ), acc[a][b]);
         constexpr int r0 = NR * x / NM, r1 = NR * (x + 1) / NM;
-        static_for<r1 - r0>([&](auto r_c) { read(std::integral_constant<int, r0 + decltype(r_c)::value>{}, Next{}, next); });
+        static_for<r1 - r0>([&](auto r_c) { read(std::integral_constant<int, r0 + decltype(r_c)::value>{}, Next{}, next, s_next); });
         constexpr int d0 = REFILL ? NLOAD * x / NM : 0, d1 = REFILL ? NLOAD * (x + 1) / NM : 0;
-        static_for<d1 - d0>([&](auto i_c) { issue(std::integral_constant<int, d0 + decltype(i_c)::value>{}, kt + NS, slot); });
+        static_for<d1 - d0>([&](auto i_c) { issue(std::integral_constant<int, d0 + decltype(i_c)::value>{}, kt + NS, slot, s_last); });
         if constexpr (F8 && x >= 2) add(std::integral_constant<int, x - 2>{});
+        // (behind the last use of tile a - 2's, whose registers these are)
+        if constexpr (F8 && !SU && x >= 2 && (x - 2) % TQ == TQ - 1 && (x - 2) / TQ + 2 < TP) sr[(x - 2) / TQ & 1] = *(const v4f *)(rows + 16 * ((x - 2) / TQ + 2));
+        if constexpr (F8 && !SU && x == 0 && TP > 1) sr[1] = *(const v4f *)(rows + 16);
         __builtin_amdgcn_sched_barrier(0);
       });
       if constexpr (F8 && NM >= 2) add(std::integral_constant<int, NM - 2>{});
       if constexpr (F8) add(std::integral_constant<int, NM - 1>{});
       slot = next;
+      s_slot = s_next;
     };
     using C0 = std::integral_constant<int, 0>;
     using C1 = std::integral_constant<int, 1>;

@@ -25,19 +25,16 @@ namespace zluda_amd {
 
 constexpr int kGradSlot = 2 * (kGradTile / 8 * (kMcPitch / 16));  // 16-byte words of a stage, the larger form
 
+// the tile whose first row and column are p0 and q0, over share z of K
 template <class E, bool QMC>
-__device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t id, v4i *lds) {
+__device__ __forceinline__ void grad_product_at(const GradProduct &g, int p0, int q0, int z, v4i *lds) {
   constexpr int B = kGradTile, WP = 2, WQ = 2, NW = WP * WQ, TP = B / WP / 16, TQ = B / WQ / 16;
   constexpr int SLOT = kGradSlot, Q_AT = SLOT / 2;  // Q in a slot
   constexpr int PASS = 8 * NW;                      // rows along K that an instruction of all waves fills
   static_assert(B / 2 == 16 * NW && B / PASS == 4, "four instructions an operand and stage");
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int wp = wave % WP, wq = wave / WP, r16 = lane & 15, g4 = lane >> 4;
-  MfmaParams at;
-  at.tiles_p = g.tiles_p; at.tiles_q = g.tiles_q; at.g.batch = 1; at.splits = g.splits; at.group_p = 8;
-  const WorkItem item = work_item(at, id);
-  const int p0 = item.p * B, q0 = item.q * B;
-  const int k0 = item.z * g.split_stages * kGradStage, k_local = min(g.k - k0, g.split_stages * kGradStage);
+  const int k0 = z * g.split_stages * kGradStage, k_local = min(g.k - k0, g.split_stages * kGradStage);
   const int stages = (k_local + kGradStage - 1) / kGradStage;
 
   // ---- DMA: a wave instruction fills 1 KiB; wave w the blocks w, w + NW, .. ----------------------------------------------------------
@@ -140,7 +137,7 @@ __device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t
   const int pc = p0 + wp * TP * 16, qc = q0 + wq * TQ * 16;
   if (g.splits > 1) {
     const int64_t pitch = (int64_t)g.tiles_p * B, plane = pitch * g.tiles_q * B;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(g.part + item.z * plane + qc * pitch + pc), 0, 0xFFFFFFFF, 0x00020000);
+    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(g.part + z * plane + qc * pitch + pc), 0, 0xFFFFFFFF, 0x00020000);
     const int vo = (r16 * (int)pitch + 4 * g4) * 4;
 #pragma unroll
     for (int a = 0; a < TP; a++)
@@ -166,6 +163,14 @@ __device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t
 #endif
       buffer_store_b128_guarded(out, rs, pc + a * 16 + first < g.np ? vo : kStoreNowhere, (b * 16 * (int)g.ldd + a * 16) * 2);
     }
+}
+
+template <class E, bool QMC>
+__device__ __forceinline__ void grad_product_tile(const GradProduct &g, uint32_t id, v4i *lds) {
+  MfmaParams at;
+  at.tiles_p = g.tiles_p; at.tiles_q = g.tiles_q; at.g.batch = 1; at.splits = g.splits; at.group_p = 8;
+  const WorkItem item = work_item(at, id);
+  grad_product_at<E, QMC>(g, item.p * kGradTile, item.q * kGradTile, item.z, lds);
 }
 
 // 64 columns of the bias gradient: every fourth row to a wave, then the four sums in order.  (A launch of its own for it takes 4 us.)

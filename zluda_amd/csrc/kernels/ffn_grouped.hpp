@@ -20,6 +20,8 @@ struct RowTile {
   int first, n;   // the expert's rows
   int at;         // the tile's first one among them
 };
+// Sums of tile counts stop here: what `offsets` should not hold overflows nothing.  (A grid has fewer tiles.)
+constexpr int kMostTiles = 1 << 30;
 // Tile `slot` of `side` rows; every wave finds it for itself (all lanes active)
 __device__ __forceinline__ RowTile find_row_tile(const int32_t *offsets, int experts, int rows, int side, int slot) {
   RowTile r{-1, 0, 0, 0};
@@ -32,7 +34,7 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t *offsets, int exp
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int t = __shfl_up(up_to, d, 64);
-      if (lane >= d) up_to += t;
+      if (lane >= d) up_to = min(up_to + t, kMostTiles);
     }
     const uint64_t past = __ballot(before + up_to > slot);
     if (past) {
@@ -43,9 +45,21 @@ __device__ __forceinline__ RowTile find_row_tile(const int32_t *offsets, int exp
       r.at = (slot - before - (__builtin_amdgcn_readlane(up_to, l) - __builtin_amdgcn_readlane(tiles, l))) * side;
       return r;
     }
-    before += __builtin_amdgcn_readlane(up_to, 63);
+    before = min(before + __builtin_amdgcn_readlane(up_to, 63), kMostTiles);
   }
   return r;
+}
+
+// How many tiles of `side` rows there are, up to `most` of them
+__device__ __forceinline__ int count_row_tiles(const int32_t *offsets, int experts, int rows, int side, int most) {
+  int all = 0;
+  for (int base = 0; base < experts; base += 64) {
+    int first;
+    all = min(all + (int)(((uint32_t)expert_rows(offsets, experts, rows, base + (threadIdx.x & 63), first) + side - 1) / (uint32_t)side), most);
+  }
+#pragma unroll
+  for (int d = 32; d; d >>= 1) all = min(all + __shfl_xor(all, d, 64), most);
+  return __builtin_amdgcn_readfirstlane(all);
 }
 
 struct GroupedParams {

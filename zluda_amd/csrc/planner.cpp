@@ -833,6 +833,7 @@ static void fill_block_plan(const Lowered &l, int variant, uint32_t cus, uint64_
   plan->grid_x = ceil_div(np, v.bp) * ceil_div(nq, v.bq); plan->grid_y = g.batch; plan->grid_z = 1;
   plan->block = v.wp * v.wq * 64;
   plan->workspace = 0;
+  // K shared out over workgroups where the tiles leave half of the chip idle: at least four stages each, and a second kernel
   const uint64_t tiles = (uint64_t)plan->grid_x * plan->grid_y, stages = (uint64_t)blocks128(g.K);
   if (tiles * 2 <= cus && stages >= 8) {
     uint64_t s = std::min<uint64_t>({8, cus / tiles, stages / 4});
@@ -847,13 +848,21 @@ static void fill_block_plan(const Lowered &l, int variant, uint32_t cus, uint64_
 }
 
 static int pick_block_variant(const Lowered &l, uint32_t cus, uint64_t workspace_size) {
-  const GemmArgs &g = l.g;
-  const uint32_t np = g.d_si != 1 ? g.N : g.M, nq = g.d_si != 1 ? g.M : g.N;
-  auto tiles = [&](int v) { return (uint64_t)ceil_div(np, kBlockVariants[v].bp) * ceil_div(nq, kBlockVariants[v].bq) * g.batch; };
-  if (nq <= 32) return 3;
-  if (block_exact(l)) return 2;
-  if (block_uniform_p(l) && tiles(0) >= cus) return 0;
-  return tiles(1) >= cus ? 1 : 2;
+  int best = -1;
+  float best_us = 0.0f;
+  for (int v = 0; v < kNumBlockVariants; v++) {
+    if ((kBlockVariants[v].uniform && !block_uniform_p(l)) || (!kBlockVariants[v].exact && block_exact(l))) continue;
+    zluda_gemm_plan p;
+    memset(&p, 0, sizeof(p));
+    fill_block_plan(l, v, cus, workspace_size, &p);
+    float us = block_tiles_us(v, (uint64_t)p.grid_x * p.grid_y * p.grid_z, ((uint64_t)blocks128(l.g.K) + p.grid_z - 1) / p.grid_z, cus, true);
+    if (p.grid_z > 1) us += 3.0f + (float)p.workspace * 2 / 3e6f;
+    if (best < 0 || us < best_us) {
+      best = v;
+      best_us = us;
+    }
+  }
+  return best;
 }
 
 uint32_t transposing_under_generic(const Lowered &l) {

@@ -2,6 +2,7 @@
 #pragma once
 #include "../../include/cublaslt_abi.h"
 #include "../../include/zluda_gemm_launch.h"
+#include "block_cost.hpp"
 #include "gemm_args.hpp"
 
 namespace zluda_amd {
@@ -55,12 +56,10 @@ constexpr int tr_ring_stages(int variant, uint64_t groups, uint64_t cus) {
 // stages of 128 K bytes; uniform: only for P rows that share their scales (the accumulators of a wave leave no registers for more); exact: also for results in
 // 32 bits (the widened operands take registers)
 struct BlockVariant { int bp, bq, wp, wq, stages; bool uniform, exact; };
-constexpr BlockVariant kBlockVariants[] = {
-    {256, 256, 2, 4, 2, true, false},   // 0
-    {128, 128, 2, 2, 2, false, false},  // 1: two workgroups per CU
-    {64, 64, 2, 2, 4, false, true},     // 2: two
-    {64, 32, 2, 2, 4, false, true},     // 3: three
-};
+constexpr BlockVariant block_variant(int v, bool uniform, bool exact) {
+  return {kBlockTiles[v].bp, kBlockTiles[v].bq, kBlockTiles[v].wp, kBlockTiles[v].wq, kBlockTiles[v].stages, uniform, exact};
+}
+constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true)};
 constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
 constexpr int kNumTrVariants = sizeof(kTrVariants) / sizeof(kTrVariants[0]);
 
