@@ -26,8 +26,10 @@ inline uint32_t launch_block_variant(const MfmaParams &prm, const zluda_gemm_pla
   case 1: return with(std::integral_constant<int, 1>{});
   case 2: return with(std::integral_constant<int, 2>{});
   case 3: return with(std::integral_constant<int, 3>{});
+  case 4: return with(std::integral_constant<int, 4>{});
+  case 5: return with(std::integral_constant<int, 5>{});
   }
-  static_assert(kNumBlockVariants == 4, "a case each");
+  static_assert(kNumBlockVariants == 6, "a case each");
   return CUBLAS_STATUS_INVALID_VALUE;
 }
 

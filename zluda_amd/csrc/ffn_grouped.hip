@@ -3,6 +3,7 @@
 
 #include "ffn_checks.hpp"
 #include "ffn_grouped_launch.hpp"
+#include "planner.hpp"
 
 using namespace zluda_amd;
 
@@ -66,14 +67,16 @@ bool tile_operands(const zluda_ffn_grouped *p) {
 }
 
 // The tile whose last workgroup is done first, if the rows are shared out about evenly, which only the device knows: a tile for each expert, and beyond that half
-// of one that is not full for each.  Measured, us, in the order of kBlockTiles: 2048 of model, 5632 features, eight experts, bf16, 16 rows 56, 42, 37, 35; 256 61,
-// 45, 39, 42; 512 62, 48, 50, 54; 2048 96, 82, 105, 126; 4096 117, 138, 172, 219; 1024 of model, 2816 features, 64 experts, 1024 rows 91, 77, 76, 71; 4096 106, 91, 97, 105.
+// of one that is not full for each.  Measured, us, in the order of kBlockTiles: 2048 of model, 5632 features, eight experts, bf16, 16 rows 53, 42, 37, 35, 39 and 46; 256 58,
+// 45, 39, 41, 42 and 48; 1024 65, 68, 66, 78, 59, 59; 2048 94, 83, 108, 129, 91, 84; 4096 118, 140, 174, 220, 148, 142; 1024 of model, 2816 features, 64 experts, 4096 rows
+// 103, 91, 97, 105, 87, 93.
 int pick_tile(const zluda_ffn_grouped *p) {
   const bool eight = p->x.type == CUDA_R_8F_E4M3, exact = eight && p->y.type == CUDA_R_32F;
   const uint64_t live = std::min(p->rows, p->experts), stages = (p->model * (eight ? 1 : 2) + 127) / 128;
   int best = -1;
   float best_us = 0.0f;
-  for (int v = exact ? 2 : 0; v < kBlockTileCount; v++) {
+  for (int v = 0; v < kBlockTileCount; v++) {
+    if (exact && !kBlockVariants[v].exact) continue;
     const uint64_t q = std::max<uint64_t>(live, p->rows / kBlockTiles[v].bq + (live + 1) / 2);
     const float us = block_tiles_us(v, q * ((p->features + kBlockTiles[v].bp - 1) / kBlockTiles[v].bp), stages, (uint64_t)cus(), eight);
     if (best < 0 || us < best_us) {

@@ -31,6 +31,10 @@ uint32_t launch_grouped(const GroupedParams &p, int tile, hipStream_t s) {
     break;
   case 2: return launch_grouped_tile<KIND, DT, 2>(p, s);
   case 3: return launch_grouped_tile<KIND, DT, 3>(p, s);
+  case 4: return launch_grouped_tile<KIND, DT, 4>(p, s);
+  case 5:
+    if constexpr (KIND != KIND_F8_WIDE) return launch_grouped_tile<KIND, DT, 5>(p, s);
+    break;
   }
   return CUBLAS_STATUS_INTERNAL_ERROR;
 }

@@ -320,6 +320,16 @@ struct WideTile {
     static_for<NLOAD>([&](auto i_c) { issue(i_c, 0, 0); });
     static_for<NLOAD>([&](auto i_c) { issue(i_c, 1, 1); });
     wait_vmcnt_barrier<0>();
+    // A wave whose share lies past the end of P or Q brings its part of the stages and meets the others, no more: the waves beside it on its SIMD have the
+    // matrix unit to themselves (a tile of at most 128 rows of Q takes little more than half the time).
+    if (wp * 128 >= P.rows || wq * 64 >= Q.rows) {
+      for (int kt = 0; kt < stages; kt++) {
+        wait_vmcnt_barrier<0>();
+        static_for<NLOAD>([&](auto i_c) { issue(i_c, kt + 2, kt & 1); });
+      }
+      __builtin_amdgcn_s_waitcnt(0);
+      return;
+    }
     static_for<8>([&](auto r_c) { read_p(C0{}, r_c, 0); });
     static_for<4>([&](auto r_c) { read_q(C0{}, r_c, 0); });
     if constexpr (F8) static_for<TQ + 1>([&](auto r_c) { read_s(r_c, 0); });

@@ -59,7 +59,9 @@ struct BlockVariant { int bp, bq, wp, wq, stages; bool uniform, exact; };
 constexpr BlockVariant block_variant(int v, bool uniform, bool exact) {
   return {kBlockTiles[v].bp, kBlockTiles[v].bq, kBlockTiles[v].wp, kBlockTiles[v].wq, kBlockTiles[v].stages, uniform, exact};
 }
-constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true)};
+constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true),
+                                           block_variant(4, false, true), block_variant(5, false, false)};
+static_assert(sizeof(kBlockVariants) / sizeof(kBlockVariants[0]) == kBlockTileCount, "a variant each");
 constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
 constexpr int kNumTrVariants = sizeof(kTrVariants) / sizeof(kTrVariants[0]);
 
