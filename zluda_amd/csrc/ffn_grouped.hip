@@ -87,6 +87,22 @@ int pick_tile(const zluda_ffn_grouped *p) {
   return best;
 }
 
+// Tiles of 128 x 128, two workgroups a CU, or of 256 x 256, whichever grad_together_stages() has done first; a stage takes 1.0 and 1.65 us.  Measured, us: 2048 of model, 5632 features,
+// eight experts, 64 rows 106 and 148, 1024 126 and 160, 4096 261 and 223, 16384 821 and 668; 1024 x 2816, 64 experts, 4096 rows 213 and 210, 16384 356 and 309; 1024 x 1024,
+// two, 8000 63 and 79; 512 x 2048, 16, 16384 101 and 82.
+int pick_grad_side(const zluda_ffn_grouped_grad *p) {
+  double us[2];
+  for (int v = 0; v < 2; v++) {
+    const uint64_t side = v ? 256 : 128, slots = (uint64_t)cus() * (v ? 1 : 2), live = std::max<uint64_t>(1, std::min(p->rows, p->experts));
+    auto tiles = [&](uint64_t n) { return (n + side - 1) / side; };
+    auto stages = [](uint64_t k) { return (k + kGradStage - 1) / kGradStage; };
+    const uint64_t n_dx = p->dx.data ? tiles(p->model) * std::max<uint64_t>(live, p->rows / side + (live + 1) / 2) : 0;
+    const uint64_t n_dw = p->dw.data ? tiles(p->model) * tiles(p->features) * p->experts : 0;
+    us[v] = grad_together_stages(slots, n_dx, stages(p->features), n_dw, stages(p->rows / p->experts), 1, 1) * (v ? 1.65 : 1.0);
+  }
+  return us[1] < us[0] ? 256 : 128;
+}
+
 // the same for the gradients, through windows of 2 GiB on an expert's matrices and rows; whole pieces of eight along every row
 bool tile_operands(const zluda_ffn_grouped_grad *p) {
   uintptr_t at = (uintptr_t)p->dy.data;
@@ -130,14 +146,15 @@ extern "C" uint32_t zluda_ffn_grouped_backward(const zluda_ffn_grouped_grad *p, 
   if (!zluda_gemm_device_cu_count()) return CUBLAS_STATUS_NOT_INITIALIZED;
   const hipStream_t s = (hipStream_t)stream;
   if (tile_operands(p)) {
-    auto tiles = [](uint64_t n) { return (n + kGradTile - 1) / kGradTile; };
-    const uint64_t dx = p->dx.data && p->rows ? tiles(p->model) * most_row_tiles(p->rows, p->experts, kGradTile) : 0;
+    const uint64_t side = (uint64_t)pick_grad_side(p);
+    auto tiles = [&](uint64_t n) { return (n + side - 1) / side; };
+    const uint64_t dx = p->dx.data && p->rows ? tiles(p->model) * most_row_tiles(p->rows, p->experts, side) : 0;
     const uint64_t dw = p->dw.data ? tiles(p->model) * tiles(p->features) * p->experts : 0;
     if (dx + dw == 0) return CUBLAS_STATUS_SUCCESS;
     if (dx + dw < (1ull << 31)) {
       const GroupedGradParams q{p->offsets, p->dy.data, p->x.data, p->w.data, p->dx.data, p->dw.data, p->dx.ld, p->dw.ld, (int32_t)p->dy.ld, (int32_t)p->x.ld, (int32_t)p->w.ld,
                                 (int32_t)p->rows, (int32_t)p->experts, (int32_t)p->features, (int32_t)p->model, (uint32_t)dx};
-      return launch_grouped_grad(q, p->dy.type, (uint32_t)(dx + dw), s);
+      return launch_grouped_grad(q, p->dy.type, (int)side, (uint32_t)(dx + dw), s);
     }
   }
   GroupedParams g{p->offsets, p->dy.data, p->w.data, p->dx.data, nullptr, nullptr, p->dy.ld, p->w.ld, p->dx.ld, 0, 0, (int32_t)p->rows, (int32_t)p->experts,

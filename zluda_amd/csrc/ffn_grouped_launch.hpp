@@ -1,7 +1,7 @@
 // Launchers of the products grouped by expert, one translation unit per kind of operands.
 #pragma once
 #include "block_cost.hpp"
-#include "kernels/ffn_grouped_tile.hpp"
+#include "kernels/ffn_grouped_grad.hpp"
 #include "launch_util.hpp"
 
 namespace zluda_amd {
@@ -12,7 +12,8 @@ inline uint64_t most_row_tiles(uint64_t rows, uint64_t experts, uint64_t side) {
 uint32_t launch_grouped_bf16(const GroupedParams &p, int tile, hipStream_t s);
 uint32_t launch_grouped_f16(const GroupedParams &p, int tile, hipStream_t s);
 uint32_t launch_grouped_f8(const GroupedParams &p, int tile, hipStream_t s);
-uint32_t launch_grouped_grad(const GroupedGradParams &p, uint32_t type, uint32_t groups, hipStream_t s);
+// side: of a tile, 128 or 256
+uint32_t launch_grouped_grad(const GroupedGradParams &p, uint32_t type, int side, uint32_t groups, hipStream_t s);
 
 template <int KIND, int DT, int V>
 uint32_t launch_grouped_tile(const GroupedParams &p, hipStream_t s) {

@@ -70,47 +70,4 @@ __global__ __launch_bounds__(WP *WQ * 64, 2) void grouped_tile_kernel(GroupedPar
   else mfma16_store_f<KIND_F8, WP, WQ, TP, TQ, DT, ACT_NONE, true>(d, acc, p0, q0, p.features, it.rows.n, 0, wave);
 }
 
-// The gradients in tiles of 128 x 128, both in one launch (ffn_grad_products.hpp: the same tiles): dX^T [model][row] = sum over features of W_e dY, dW_e^T [model][feature] =
-// sum over the expert's rows of X dY.
-struct GroupedGradParams {
-  const int32_t *offsets;
-  const void *dy, *x, *w;
-  void *dx, *dw;                 // or NULL
-  int64_t lddx, lddw;
-  int32_t lddy, ldx, ldw;
-  int32_t rows, experts, features, model;
-  uint32_t dx_groups;            // workgroups of dx, the first ones
-};
-template <class E>
-__global__ __launch_bounds__(256, 2) void grouped_grad_kernel(GroupedGradParams p) {
-  __shared__ v4i lds[2 * kGradSlot];
-  using raw = typename E::raw;
-  const int tiles_m = (p.model + kGradTile - 1) / kGradTile;
-  GradProduct g;
-  g.part = nullptr; g.splits = 1; g.np = p.model; g.tiles_p = tiles_m;
-  if (blockIdx.x < p.dx_groups) {
-    GroupedParams q;
-    q.offsets = p.offsets; q.experts = p.experts; q.rows = p.rows;
-    const GroupedItem it = grouped_item(q, tiles_m, kGradTile, blockIdx.x, p.dx_groups);
-    if (it.rows.e < 0) return;
-    g.p = (const raw *)p.w + (int64_t)it.rows.e * p.features * p.ldw; g.ldp = p.ldw;
-    g.q = (const raw *)p.dy + (int64_t)it.rows.first * p.lddy; g.ldq = p.lddy;
-    g.d = (raw *)p.dx + it.rows.first * p.lddx; g.ldd = p.lddx;
-    g.nq = it.rows.n; g.k = p.features; g.split_stages = (g.k + kGradStage - 1) / kGradStage;
-    grad_product_at<E, false>(g, it.p * kGradTile, it.rows.at, 0, lds);
-    return;
-  }
-  const int tiles_f = (p.features + kGradTile - 1) / kGradTile;
-  MfmaParams at;
-  at.tiles_p = tiles_m; at.tiles_q = tiles_f; at.g.batch = p.experts; at.splits = 1; at.group_p = 8;
-  const WorkItem item = work_item(at, blockIdx.x - p.dx_groups);
-  int first;
-  const int n = expert_rows(p.offsets, p.experts, p.rows, item.bt, first);
-  g.p = (const raw *)p.x + (int64_t)first * p.ldx; g.ldp = p.ldx;
-  g.q = (const raw *)p.dy + (int64_t)first * p.lddy; g.ldq = p.lddy;
-  g.d = (raw *)p.dw + (int64_t)item.bt * p.features * p.lddw; g.ldd = p.lddw;
-  g.nq = p.features; g.k = n; g.split_stages = (n + kGradStage - 1) / kGradStage;
-  grad_product_at<E, true>(g, item.p * kGradTile, item.q * kGradTile, 0, lds);
-}
-
 } // namespace zluda_amd
