@@ -6,8 +6,9 @@ namespace zluda_amd {
 
 // Tiles of P x Q rows, waves along each, LDS stages of 128 bytes of K.  Of them a CU holds `per_cu` workgroups, and n of those take base + n * slope us a
 // stage (8-bit operands with their scales, 16-bit ones).  Measured on whole calls over 2048 of model, 5632 features, 16384 rows of eight experts: 8-bit 213, 259, 413,
-// 533, 289 and 302 us, 16-bit 354, 441, 597, 764, 506 and 453; and on calls that leave a CU one workgroup: 333 tokens, 5632 x 2000 32, 18.5, 19.0, 18.4, 18.0 and 15.8,
-// 1000, 2048 x 2048 26.5, 18.0, 11.6, 15.2, 10.4 and 17.8.
+// 533, 289 and 302 us, 16-bit 354, 441, 597, 764, 506 and 453 (the first six); and on calls that leave a CU one workgroup: 333 tokens, 5632 x 2000 31, 18.3, 17.9, 18.2,
+// 17.2, 15.5 and 13.9, 1000, 2048 x 2048 26.5, 18.0, 11.4, 15.2, 10.4, 17.7 and 12.1, 700, 4096 x 4096 -, 25.9, 26.7, -, 22.0, 21.9 and 19.8.  (The last shape is there for
+// what 128 x 128 leaves idle: 132 tiles of 5632 x 333 on 256 CUs are 176 of 96 columns.)
 struct BlockTile { int bp, bq, wp, wq, stages, per_cu; float base8, slope8, base16, slope16; };
 constexpr BlockTile kBlockTiles[] = {
     {256, 256, 2, 4, 2, 1, 0.0f, 1.82f, 0.0f, 1.69f},
@@ -16,8 +17,9 @@ constexpr BlockTile kBlockTiles[] = {
     {64, 32, 2, 2, 4, 3, 0.13f, 0.108f, 0.13f, 0.08f},
     {128, 64, 2, 2, 3, 2, 0.05f, 0.33f, 0.05f, 0.31f},
     {128, 128, 2, 2, 4, 1, 0.0f, 0.67f, 0.0f, 0.56f},
+    {128, 96, 2, 2, 4, 1, 0.0f, 0.53f, 0.0f, 0.45f},
 };
-constexpr int kBlockTileCount = 6;
+constexpr int kBlockTileCount = 7;
 
 // us until `tiles` workgroups of tile v are done on `cus` CUs, each with `stages` of K and the time of three for its start and end
 inline float block_tiles_us(int v, uint64_t tiles, uint64_t stages, uint64_t cus, bool eight_bits) {

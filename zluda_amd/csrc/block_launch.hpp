@@ -1,5 +1,6 @@
 // Launchers of the products with a scale for each 128 of K; one translation unit per pair of formats.
 #pragma once
+#include "kernels/block_decode.hpp"
 #include "kernels/block_gemm.hpp"
 #include "launch_util.hpp"
 #include "planner.hpp"
@@ -14,6 +15,8 @@ inline uint32_t launch_block_variant(const MfmaParams &prm, const zluda_gemm_pla
     constexpr BlockVariant v = kBlockVariants[decltype(v_c)::value];
     constexpr bool U = decltype(uniform_c)::value, X = decltype(exact_c)::value;
     if constexpr ((X && !v.exact) || (!U && v.uniform)) return CUBLAS_STATUS_INVALID_VALUE;
+    else if constexpr (decltype(v_c)::value == kBlockDecode)
+      return launch_kernel(block_decode_kernel<FP, FQ, U, X>, grid, dim3(512), s, prm);
     else return launch_kernel(block_gemm_kernel<FP, FQ, U, X, v.bp, v.bq, v.wp, v.wq, v.stages>, grid, dim3(v.wp * v.wq * 64), s, prm);
   };
   auto with = [&](auto v_c) -> uint32_t {
@@ -28,8 +31,10 @@ inline uint32_t launch_block_variant(const MfmaParams &prm, const zluda_gemm_pla
   case 3: return with(std::integral_constant<int, 3>{});
   case 4: return with(std::integral_constant<int, 4>{});
   case 5: return with(std::integral_constant<int, 5>{});
+  case 6: return with(std::integral_constant<int, 6>{});
+  case kBlockDecode: return with(std::integral_constant<int, kBlockDecode>{});
   }
-  static_assert(kNumBlockVariants == 6, "a case each");
+  static_assert(kNumBlockVariants == 8, "a case each");
   return CUBLAS_STATUS_INVALID_VALUE;
 }
 

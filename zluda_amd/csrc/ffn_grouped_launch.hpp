@@ -36,6 +36,9 @@ uint32_t launch_grouped(const GroupedParams &p, int tile, hipStream_t s) {
   case 5:
     if constexpr (KIND != KIND_F8_WIDE) return launch_grouped_tile<KIND, DT, 5>(p, s);
     break;
+  case 6:
+    if constexpr (KIND != KIND_F8_WIDE) return launch_grouped_tile<KIND, DT, 6>(p, s);
+    break;
   }
   return CUBLAS_STATUS_INTERNAL_ERROR;
 }

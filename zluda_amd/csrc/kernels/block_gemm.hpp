@@ -21,6 +21,7 @@ __device__ __forceinline__ void block_sides(const MfmaParams &prm, int p0, int q
     s.scales = s.per_row ? scales + r0 : scales + (r0 >> 7) * line;
     s.s_row = s.per_row ? 1 : (int)line;
     s.s_step = s.per_row ? all : 1;
+    s.s_at = r0 & 127;
     return s;
   };
   P = side(!prm.swapped, p0);

@@ -44,6 +44,7 @@ struct TileSide {
   const float *scales;  // of the first row in the first block; unused by 16-bit kinds
   int s_row, s_step;    // floats from row to row (per_row) or from 128 rows to the next 128; from a block of K to the next
   bool per_row;
+  int s_at;             // the first row's place in its block of 128 (tiles of 96 rows begin anywhere)
 };
 
 // 8-bit floats widened to bf16, which holds them exactly, for results in 32 bits.  The 8-bit instruction does not keep 32 bits inside: of each eight
@@ -80,7 +81,7 @@ template <int KIND, int FP, int FQ, bool SU, int BP, int BQ, int WP, int WQ, int
 struct RingTile {
   static constexpr bool F8 = kind_is_block8(KIND), EXACT = KIND == KIND_F8_WIDE;
   static constexpr int NW = WP * WQ, RPP = 8 * NW, LP = BP / RPP, LQ = BQ / RPP;
-  static constexpr int SP = BP < 64 ? 64 : BP, SQ = BQ < 64 ? 64 : BQ, PIECES = (SP + SQ) / 64, LS = F8 ? (PIECES + NW - 1) / NW : 0;
+  static constexpr int SP = (BP + 63) / 64 * 64, SQ = (BQ + 63) / 64 * 64, PIECES = (SP + SQ) / 64, LS = F8 ? (PIECES + NW - 1) / NW : 0;
   static constexpr int NLOAD = LP + LQ + LS;
   static constexpr int TP = BP / WP / 16, TQ = BQ / WQ / 16;
   // 16-byte words: the slots, behind them the scales of one stage more than there are slots (those of P's rows are read while their stage is multiplied, when its
@@ -116,7 +117,7 @@ struct RingTile {
       const int piece = (wave + NW * i) % PIECES;
       const TileSide &side = piece < SP / 64 ? P : Q;
       const int row = min((piece < SP / 64 ? piece : piece - SP / 64) * 64 + lane, min(piece < SP / 64 ? BP : BQ, side.rows) - 1);
-      os[i] = (side.per_row ? row * side.s_row : (row >> 7) * side.s_row) * 4;
+      os[i] = (side.per_row ? row : (row + side.s_at) >> 7) * side.s_row * 4;
     }
     auto issue = [&](auto i_c, int kt, int slot, int s_slot) __attribute__((always_inline)) {  // instruction i of a stage
       constexpr int i = decltype(i_c)::value;

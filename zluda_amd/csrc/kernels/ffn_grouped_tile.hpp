@@ -43,8 +43,8 @@ __global__ __launch_bounds__(WP *WQ * 64, 2) void grouped_tile_kernel(GroupedPar
   Q.data = (const uint8_t *)p.a + ((int64_t)it.rows.first + q0) * p.lda * ESZ;
   Q.ld = (int)p.lda * ESZ;
   Q.rows = it.rows.n - q0;
-  P.scales = p.b_scales; P.s_row = P.s_step = 0; P.per_row = false;
-  Q.scales = p.a_scales; Q.s_row = Q.s_step = 0; Q.per_row = true;
+  P.scales = p.b_scales; P.s_row = P.s_step = 0; P.per_row = false; P.s_at = p0 & 127;
+  Q.scales = p.a_scales; Q.s_row = Q.s_step = 0; Q.per_row = true; Q.s_at = 0;
   if constexpr (F8) {
     P.scales += ((int64_t)it.rows.e * ((p.features + 127) >> 7) + (p0 >> 7)) * p.ldb_scales;
     P.s_row = (int)p.ldb_scales; P.s_step = 1;

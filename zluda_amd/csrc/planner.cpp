@@ -835,7 +835,7 @@ static void fill_block_plan(const Lowered &l, int variant, uint32_t cus, uint64_
   plan->workspace = 0;
   // K shared out over workgroups where the tiles leave half of the chip idle: at least four stages each, and a second kernel
   const uint64_t tiles = (uint64_t)plan->grid_x * plan->grid_y, stages = (uint64_t)blocks128(g.K);
-  if (tiles * 2 <= cus && stages >= 8) {
+  if (variant != kBlockDecode && tiles * 2 <= cus && stages >= 8) {
     uint64_t s = std::min<uint64_t>({8, cus / tiles, stages / 4});
     const uint64_t each = (uint64_t)g.batch * ceil_div(np, v.bp) * v.bp * ceil_div(nq, v.bq) * v.bq * 4;
     while (s > 1 && s * each > workspace_size) s--;
@@ -847,10 +847,21 @@ static void fill_block_plan(const Lowered &l, int variant, uint32_t cus, uint64_
   plan->waves = (float)(tiles * plan->grid_z) / (float)cus;
 }
 
+// The kernel that shares K out inside a workgroup for up to 16 tokens, where its waves have two blocks of K each at most and its workgroups are one round.  Measured
+// against tiles that share K out over workgroups, with their second kernel (us in a graph; one token, 128 x 128 a scale): 256 x 1024 4.8 and 5.8, 2048 x 2048 5.3 and
+// 6.3, 1024 x 4096 6.1 and 6.4; beyond, 5632 x 2048 8.3 and 7.6, 2048 x 8192 9.1 and 8.3, 14336 x 4096 17.5 and 11.3 (16 tokens 5.1 and 6.1, 6.0 and 6.5, 7.3 and 6.7,
+// 9.6 and 7.9, 11.2 and 8.5, 21.7 and 11.5): loads into registers reach less of the memory's rate than those into LDS.  Called one at a time the second
+// kernel costs 2.3 us more: 2048 x 2048 7.6 and 9.9.
+static bool block_decode_pays(const Lowered &l, uint32_t cus) {
+  const uint32_t np = l.g.d_si != 1 ? l.g.N : l.g.M, nq = l.g.d_si != 1 ? l.g.M : l.g.N;
+  return nq <= 16 && blocks128(l.g.K) <= 16 && (uint64_t)ceil_div(np, 16) * l.g.batch <= cus;
+}
+
 static int pick_block_variant(const Lowered &l, uint32_t cus, uint64_t workspace_size) {
+  if (block_decode_pays(l, cus)) return kBlockDecode;
   int best = -1;
   float best_us = 0.0f;
-  for (int v = 0; v < kNumBlockVariants; v++) {
+  for (int v = 0; v < kBlockTileCount; v++) {
     if ((kBlockVariants[v].uniform && !block_uniform_p(l)) || (!kBlockVariants[v].exact && block_exact(l))) continue;
     zluda_gemm_plan p;
     memset(&p, 0, sizeof(p));

@@ -60,8 +60,10 @@ constexpr BlockVariant block_variant(int v, bool uniform, bool exact) {
   return {kBlockTiles[v].bp, kBlockTiles[v].bq, kBlockTiles[v].wp, kBlockTiles[v].wq, kBlockTiles[v].stages, uniform, exact};
 }
 constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true),
-                                           block_variant(4, false, true), block_variant(5, false, false)};
-static_assert(sizeof(kBlockVariants) / sizeof(kBlockVariants[0]) == kBlockTileCount, "a variant each");
+                                           block_variant(4, false, true), block_variant(5, false, false), block_variant(6, false, false),
+                                           {16, 16, 1, 8, 0, false, true}};  // kernels/block_decode.hpp: no tile of those
+constexpr int kBlockDecode = kBlockTileCount;
+static_assert(sizeof(kBlockVariants) / sizeof(kBlockVariants[0]) == kBlockDecode + 1, "a variant each");
 constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
 constexpr int kNumTrVariants = sizeof(kTrVariants) / sizeof(kTrVariants[0]);
 
