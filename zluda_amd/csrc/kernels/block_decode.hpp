@@ -39,7 +39,7 @@ __global__ __launch_bounds__(512, 4) void block_decode_kernel(MfmaParams prm) {
   // the wave's block i, what lies past the end of K or past the last block as zeros: out of the windows, no traffic
   auto load = [&](auto j_c, int i) __attribute__((always_inline)) {
     constexpr int j = decltype(j_c)::value;
-    const int blk = wave + NW * i, at = blk * 128, none = blk < blocks ? 0 : kOut;
+    const int blk = wave + NW * i, at = blk * 128, none = blk < blocks ? 0 : kOut, s_blk = min(blk, blocks - 1);  // (uniform offsets stay within the windows)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       const int oob = at + 16 * grp + 64 * h < K ? 0 : kOut;
@@ -47,8 +47,8 @@ __global__ __launch_bounds__(512, 4) void block_decode_kernel(MfmaParams prm) {
       qf[j][h] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rq, (oq + 64 * h) | oob, at, 0));
     }
 #pragma unroll
-    for (int e = 0; e < (SU ? 1 : 4); e++) sp[j][e] = bits2f(__builtin_amdgcn_raw_buffer_load_b32(rsp, osp[e] | none, blk * P.s_step * 4, 0));
-    sq[j] = bits2f(__builtin_amdgcn_raw_buffer_load_b32(rsq, osq | none, blk * Q.s_step * 4, 0));
+    for (int e = 0; e < (SU ? 1 : 4); e++) sp[j][e] = bits2f(__builtin_amdgcn_raw_buffer_load_b32(rsp, osp[e] | none, s_blk * P.s_step * 4, 0));
+    sq[j] = bits2f(__builtin_amdgcn_raw_buffer_load_b32(rsq, osq | none, s_blk * Q.s_step * 4, 0));
   };
   v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
   static_for<AHEAD>([&](auto j_c) { load(j_c, decltype(j_c)::value); });

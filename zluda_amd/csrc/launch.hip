@@ -161,7 +161,7 @@ uint32_t launch_block(const Lowered &l, const zluda_gemm_plan &plan, void *ws, u
   if (plan.swapped != (uint32_t)(l.g.d_si != 1) || (uint32_t)(prm.tiles_p * prm.tiles_q) != plan.grid_x || (uint32_t)l.g.batch != plan.grid_y) return CUBLAS_STATUS_INVALID_VALUE;
   if (plan.grid_z > 1) {
     const uint64_t need = (uint64_t)plan.grid_z * l.g.batch * prm.tiles_p * v.bp * prm.tiles_q * v.bq * 4;
-    if (!ws || (((uintptr_t)ws) & 15) || ws_size < need || plan.workspace < need) return CUBLAS_STATUS_INVALID_VALUE;
+    if (plan.variant == kBlockDecode || !ws || (((uintptr_t)ws) & 15) || ws_size < need || plan.workspace < need) return CUBLAS_STATUS_INVALID_VALUE;
     prm.splits = (int32_t)plan.grid_z;
     prm.split_stages = (int32_t)((blocks128(l.g.K) + prm.splits - 1) / prm.splits);
     prm.ws = ws;
