@@ -5,8 +5,8 @@ import torch
 import ffn_oracle as O
 import packed_oracle as P
 from test_gpu_ffn import DEV, Mat, TYPES, randn, stream
-from test_gpu_grouped import offsets_of, pack, run_backward, run_forward, check_forward, values
-from zluda_amd import ffn
+from test_gpu_grouped import check_forward, offsets_of, pack, run_backward, run_forward, untouched
+from zluda_amd import cublaslt, ffn
 
 pytestmark = pytest.mark.gpu
 BF = TYPES["bf16"]
@@ -18,6 +18,33 @@ BF = TYPES["bf16"]
 def test_large_tiles(typ, counts, spare, f, d):
     run_backward(typ, counts, spare, f, d)
     check_forward(*run_forward(typ, counts, spare, f, d), f, "%s %dx%d" % (typ, f, d))
+
+
+@pytest.mark.parametrize("typ", ["bf16", "f16"])
+@pytest.mark.parametrize("counts,spare,f,d", [([9, 7, 8, 0, 10, 8, 14, 8], 0, 5632, 2048), ([40, 0, 37, 200], 23, 2816, 1032), ([64], 0, 4096, 4096), ([692], 8, 4744, 520),
+                                              ([3, 1], 0, 2048, 136), ([700, 1, 600, 699], 5, 4096, 512)])
+def test_shares_of_a_long_k(typ, counts, spare, f, d):
+    """few tiles of dx with a long K: shares of it, summed up behind; nothing is written past the workspace that was asked for, and less of it is refused"""
+    dt, code = TYPES[typ]
+    o, dev = offsets_of(counts)
+    rows, e = o[-1] + spare, len(counts)
+    dy, x, w = Mat(rows, f, dt, None, 0, randn(1, rows, f, std=0.1)), Mat(rows, d, dt, None, 0, randn(2, rows, d)), Mat(e * f, d, dt, None, 0, randn(3, e * f, d, std=f ** -0.5))
+    dx, dw = Mat(rows, d, dt, d + 8), Mat(e * f, d, dt)
+    call = ffn.GroupedBackward(dict(type=code, rows=rows, experts=e, features=f, model=d, lddx=dx.ld))
+    assert call.workspace > 0
+    ws = torch.full((call.workspace + 4096,), 0xCD, dtype=torch.uint8, device=DEV)
+    args = dict(offsets=dev.data_ptr(), dy=dy.ptr, x=x.ptr, w=w.ptr, dx=dx.ptr, dw=dw.ptr, stream=stream())
+    for bad in (dict(workspace=ws.data_ptr(), workspace_size=call.workspace - 1), dict(workspace=None, workspace_size=call.workspace), dict()):
+        with pytest.raises(cublaslt.CublasLtError):
+            call.run(**args, **bad)
+    call.run(**args, workspace=ws.data_ptr(), workspace_size=call.workspace)
+    torch.cuda.synchronize()
+    assert dx.guards() and dw.guards() and untouched(dx, o[-1]) and bool((ws[call.workspace:] == 0xCD).all())
+    for i in range(e):
+        r, q = slice(o[i], o[i + 1]), slice(i * f, (i + 1) * f)
+        if counts[i]:
+            O.check(dx.view[r], P.product(dy.view[r].double(), w.view[q].double().t()), "dx, expert %d" % i)
+        O.check(dw.view[q], P.product(dy.view[r].double().t(), x.view[r].double().t()), "dw, expert %d" % i)
 
 
 BAD = [float("nan"), float("inf"), -float("inf")]
@@ -32,11 +59,12 @@ def test_rows_keep_to_themselves(counts, spare, f, d, bad):
     x, dy, w = randn(1, rows, d).to(BF[0]), randn(2, rows, f).to(BF[0]), randn(3, e * f, d, std=d ** -0.5).to(BF[0])
     spec = dict(type=BF[1], rows=rows, experts=e, features=f, model=d)
     fwd, bwd = ffn.GroupedForward(spec), ffn.GroupedBackward(spec)
+    ws = torch.empty(max(16, bwd.workspace), dtype=torch.uint8, device=DEV)
 
     def run():
         y, dx, dw = torch.zeros_like(dy), torch.zeros_like(x), torch.zeros_like(w)
         fwd.run(offsets=dev.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), y=y.data_ptr(), stream=stream())
-        bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), stream=stream())
+        bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), workspace=ws.data_ptr(), workspace_size=ws.numel(), stream=stream())
         torch.cuda.synchronize()
         return y, dx, dw.view(e, f, d)
     y0, dx0, dw0 = run()
@@ -93,6 +121,7 @@ def test_gradients_of_experts_are_differences(counts, f, d):
     x, w, dy, vx, vw = ints(1, 2, rows, d), ints(2, 1, e * f, d), ints(3, 1, rows, f), ints(4, 1, rows, d), ints(5, 1, e * f, d)
     spec = dict(type=BF[1], rows=rows, experts=e, features=f, model=d)
     fwd, bwd = ffn.GroupedForward(spec), ffn.GroupedBackward(spec)
+    ws = torch.empty(max(16, bwd.workspace), dtype=torch.uint8, device=DEV)
 
     def loss(x, w):
         y = torch.empty_like(dy)
@@ -101,7 +130,7 @@ def test_gradients_of_experts_are_differences(counts, f, d):
         assert y.abs().max() <= 256                         # (integers up to here are bfloat16 values)
         return (y.double() * dy.double()).sum()
     dx, dw = torch.empty_like(x), torch.empty_like(w)
-    bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), stream=stream())
+    bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), workspace=ws.data_ptr(), workspace_size=ws.numel(), stream=stream())
     torch.cuda.synchronize()
     assert dx.abs().max() <= 256 and dw.abs().max() <= 256
     assert loss(x + vx, w) - loss(x, w) == (dx.double() * vx.double()).sum()

@@ -116,10 +116,11 @@ def grouped_pass(counts, f, d, seed):
     y, dx, dw = torch.empty_like(dy), torch.empty_like(x), torch.empty_like(w)
     spec = dict(type=BF[1], rows=rows, experts=e, features=f, model=d)
     fwd, bwd = ffn.GroupedForward(spec), ffn.GroupedBackward(spec)
+    ws = torch.empty(max(16, bwd.workspace), dtype=torch.uint8, device=DEV)
 
     def run(stream):
         fwd.run(offsets=dev.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), y=y.data_ptr(), stream=stream)
-        bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), stream=stream)
+        bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), workspace=ws.data_ptr(), workspace_size=ws.numel(), stream=stream)
 
     def check(counts, what):
         at = 0
@@ -183,7 +184,8 @@ def test_matrices_beyond_4_gib():
     dy[-150:] = randn(4, 150, f).to(BF[0])
     dx, dw = Mat(rows, d, BF[0], ld), torch.empty_like(w)
     bwd = ffn.GroupedBackward(dict(type=BF[1], rows=rows, experts=e, features=f, model=d, ldx=ld, lddx=ld))
-    bwd.run(offsets=o.data_ptr(), dy=dy.data_ptr(), x=x.ptr, w=w.data_ptr(), dx=dx.ptr, dw=dw.data_ptr(), stream=stream())
+    ws = torch.empty(max(16, bwd.workspace), dtype=torch.uint8, device=DEV)
+    bwd.run(offsets=o.data_ptr(), dy=dy.data_ptr(), x=x.ptr, w=w.data_ptr(), dx=dx.ptr, dw=dw.data_ptr(), workspace=ws.data_ptr(), workspace_size=ws.numel(), stream=stream())
     torch.cuda.synchronize()
     O.check(dx.view[-150:], P.product(dy[-150:].double(), last.double().t()), "dx")
     O.check(dw[-f:], P.product(dy[-150:].double().t(), tail.double().t()), "dw")

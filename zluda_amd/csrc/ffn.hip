@@ -203,8 +203,9 @@ uint32_t run_together(uint32_t type, const zluda_ffn_gated_grad *p, const zluda_
   const int model = (int)p->model, tokens = (int)p->tokens, f2 = (int)(2 * p->features);
   auto tiles = [](int n) { return (n + kGradTile - 1) / kGradTile; };
   GradProductsParams m;
-  m.dx = {p->w.data, g.dz, p->dx.data, part, p->dx.ld, (int32_t)p->w.ld, (int32_t)plan.lddz, model, tokens, f2, tiles(model), tiles(tokens), (int32_t)t.splits, (int32_t)t.split_stages};
-  m.dw = {x.data, g.dz, p->dw.data, nullptr, p->dw.ld, (int32_t)x.ld, (int32_t)plan.lddz, model, f2, tokens, tiles(model), tiles(f2), 1, (tokens + kGradStage - 1) / kGradStage};
+  m.dx = {p->w.data, g.dz, p->dx.data, part, p->dx.ld, (int32_t)p->w.ld, (int32_t)plan.lddz, model, tokens, f2, tiles(model), tiles(tokens), (int32_t)t.splits, (int32_t)t.split_stages,
+          (int64_t)tiles(model) * kGradTile * tiles(tokens) * kGradTile, tiles(tokens) * kGradTile};
+  m.dw = {x.data, g.dz, p->dw.data, nullptr, p->dw.ld, (int32_t)x.ld, (int32_t)plan.lddz, model, f2, tokens, tiles(model), tiles(f2), 1, (tokens + kGradStage - 1) / kGradStage, 0, 0};
   m.dx_groups = (uint32_t)(m.dx.tiles_p * m.dx.tiles_q) * t.splits;
   m.sums = g.part; m.dbias = p->dbias; m.shares = (int32_t)plan.shares;
   FFN_CHECK(launch_grad_products(type, m, s));

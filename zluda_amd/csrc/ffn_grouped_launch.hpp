@@ -12,6 +12,8 @@ inline uint64_t most_row_tiles(uint64_t rows, uint64_t experts, uint64_t side) {
 uint32_t launch_grouped_bf16(const GroupedParams &p, int tile, hipStream_t s);
 uint32_t launch_grouped_f16(const GroupedParams &p, int tile, hipStream_t s);
 uint32_t launch_grouped_f8(const GroupedParams &p, int tile, hipStream_t s);
+// the sums of dx's shares
+uint32_t launch_grouped_round(const RoundParams &r, uint32_t type, const int32_t *offsets, int32_t experts, dim3 grid, hipStream_t s);
 // side: of a tile, 128 or 256
 uint32_t launch_grouped_grad(const GroupedGradParams &p, uint32_t type, int side, uint32_t groups, hipStream_t s);
 

@@ -17,7 +17,7 @@ uint32_t launch_gated_small_f16(const GatedParams &p, int tile, hipStream_t s);
 
 // ---- the products of the backward pass in one launch (kernels/ffn_grad_products.hpp) ----------------------------------------------
 // D[q][p] = sum over k of P[k][p] Q, Q as [q][k] (dX) or [k][q] (dW).  With `splits` > 1 share z of K writes 32-bit sums to
-// part[z][q][p], q and p padded to whole tiles.
+// part[z][q][p], p padded to whole tiles, part_rows rows of q, part_plane floats from share to share.
 struct GradProduct {
   const void *p, *q;
   void *d;
@@ -26,6 +26,8 @@ struct GradProduct {
   int32_t ldp, ldq;
   int32_t np, nq, k;
   int32_t tiles_p, tiles_q, splits, split_stages;
+  int64_t part_plane;
+  int32_t part_rows;
 };
 struct GradProductsParams {
   GradProduct dx, dw;

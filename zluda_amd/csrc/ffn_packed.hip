@@ -49,7 +49,7 @@ uint32_t launch_rms(RmsParams p, hipStream_t s) {
 // shape, with one sum less
 int rms_grad_rows_each(uint64_t cols) { return cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1; }
 uint32_t rms_grad_groups(uint64_t rows, uint64_t cols) {
-  const int each = rms_grad_rows_each(cols), least = rows <= 64ull * each ? each : 2 * each;
+  const int each = rms_grad_rows_each(cols), least = rows <= (uint64_t)cus() * 7 / 8 * each ? each : 2 * each;
   if (rows <= 3ull * each) return 1;
   return (uint32_t)std::min<uint64_t>((rows + least - 1) / least, (uint64_t)cus() * (cols <= 4096 ? 2 : 1));
 }

@@ -55,10 +55,10 @@ struct RoundParams {
 
 // Sums held in 32 bits to their type: the shares of x, `plane` elements apart, added in order (rows of x on 16 bytes and padded to whole pieces)
 template <class E>
-__global__ __launch_bounds__(256) void round_rows_kernel(RoundParams p) {
+__device__ __forceinline__ void round_rows(const RoundParams &p, int64_t first, int64_t end) {
   const int col = 8 * (blockIdx.x * 64 + (threadIdx.x & 63));
   if (col >= p.cols) return;
-  for (int64_t row = blockIdx.y * 4 + (threadIdx.x >> 6); row < p.rows; row += gridDim.y * 4) {
+  for (int64_t row = first + blockIdx.y * 4 + (threadIdx.x >> 6); row < end; row += gridDim.y * 4) {
     const float *x = p.x + row * p.ldx + col;
     float v[8] = {};
 #pragma unroll 4
@@ -70,6 +70,8 @@ __global__ __launch_bounds__(256) void round_rows_kernel(RoundParams p) {
     store8<E>((typename E::raw *)p.y + row * p.ldy + col, v, p.cols - col);
   }
 }
+template <class E>
+__global__ __launch_bounds__(256) void round_rows_kernel(RoundParams p) { round_rows<E>(p, 0, p.rows); }
 
 struct GatedGradParams {
   const void *dh, *gate, *up;              // gate, up: elements or codes

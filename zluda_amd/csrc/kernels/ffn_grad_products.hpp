@@ -136,8 +136,9 @@ __device__ __forceinline__ void grad_product_at(const GradProduct &g, int p0, in
   // ---- D: a lane has P rows 4 g4 .. + 3 of a tile, column r16 ----------------------------------------------------------------------------
   const int pc = p0 + wp * TP * 16, qc = q0 + wq * TQ * 16;
   if (g.splits > 1) {
-    const int64_t pitch = (int64_t)g.tiles_p * B, plane = pitch * g.tiles_q * B;
-    const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc((void *)(g.part + z * plane + qc * pitch + pc), 0, 0xFFFFFFFF, 0x00020000);
+    const int64_t pitch = (int64_t)g.tiles_p * B, corner = qc * pitch + pc;
+    const __amdgpu_buffer_rsrc_t rs =
+        __builtin_amdgcn_make_buffer_rsrc((void *)(g.part + z * g.part_plane + corner), 0, tile_window_bytes(pitch, (int)pitch, g.part_rows, corner, 4), 0x00020000);
     const int vo = (r16 * (int)pitch + 4 * g4) * 4;
 #pragma unroll
     for (int a = 0; a < TP; a++)

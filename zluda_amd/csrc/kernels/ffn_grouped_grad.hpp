@@ -3,6 +3,7 @@
 // One operand (P: W_e or X) lies along its row index, the other (Q: dY) along K for dX and along its row index for dW, as in ffn_grad_products.hpp, whose 128 x 128
 // tiles and LDS layouts these are; and tiles of 256 x 256 on eight waves of 128 x 64, with the sub-steps of WideTile (block_tile.hpp).
 #pragma once
+#include "ffn_elementwise.hpp"
 #include "ffn_grouped_tile.hpp"
 
 namespace zluda_amd {
@@ -15,6 +16,9 @@ struct GroupedGradParams {
   int32_t lddy, ldx, ldw;
   int32_t rows, experts, features, model;
   uint32_t dx_groups;            // workgroups of dx, the first ones
+  // tiles of 128 x 128 may share out dx's K: share z of a row leaves its sums in part[z][row], whole tiles of model wide
+  float *part;
+  int32_t dx_splits, dx_split_stages;
 };
 
 // The 256 x 256 tile whose first row and column are p0 and q0.  LDS: P's two slots, Q's two, in blocks of 1 KiB at a pitch of 1056 bytes or (Q along K) eight swizzled
@@ -150,14 +154,21 @@ __global__ __launch_bounds__(B == 256 ? 512 : 256, 2) void grouped_grad_kernel(G
   if (blockIdx.x < p.dx_groups) {
     GroupedParams q;
     q.offsets = p.offsets; q.experts = p.experts; q.rows = p.rows;
-    const GroupedItem it = grouped_item(q, tiles_m, B, blockIdx.x, p.dx_groups);
+    const uint32_t tiles = B == 256 ? p.dx_groups : p.dx_groups / (uint32_t)p.dx_splits, z = B == 256 ? 0 : blockIdx.x / tiles;
+    const GroupedItem it = grouped_item(q, tiles_m, B, blockIdx.x - z * tiles, tiles);
     if (it.rows.e < 0) return;
     g.p = (const raw *)p.w + (int64_t)it.rows.e * p.features * p.ldw; g.ldp = p.ldw;
     g.q = (const raw *)p.dy + (int64_t)it.rows.first * p.lddy; g.ldq = p.lddy;
     g.d = (raw *)p.dx + it.rows.first * p.lddx; g.ldd = p.lddx;
     g.nq = it.rows.n; g.k = p.features; g.split_stages = (g.k + kGradStage - 1) / kGradStage;
-    if constexpr (B == 256) grouped_grad_wide<E, false>(g, it.p * B, it.rows.at, lds);
-    else grad_product_at<E, false>(g, it.p * B, it.rows.at, 0, lds);
+    if constexpr (B == 256) {
+      grouped_grad_wide<E, false>(g, it.p * B, it.rows.at, lds);
+    } else {
+      const int64_t pitch = (int64_t)tiles_m * B;
+      g.splits = p.dx_splits; g.split_stages = p.dx_split_stages;
+      g.part = p.part + it.rows.first * pitch; g.part_plane = p.rows * pitch; g.part_rows = g.nq;
+      grad_product_at<E, false>(g, it.p * B, it.rows.at, (int)z, lds);
+    }
     return;
   }
   MfmaParams at;
@@ -171,6 +182,12 @@ __global__ __launch_bounds__(B == 256 ? 512 : 256, 2) void grouped_grad_kernel(G
   g.nq = p.features; g.k = n; g.split_stages = (n + kGradStage - 1) / kGradStage;
   if constexpr (B == 256) grouped_grad_wide<E, true>(g, item.p * B, item.q * B, lds);
   else grad_product_at<E, true>(g, item.p * B, item.q * B, 0, lds);
+}
+
+// the shares of dx, of the rows that experts have
+template <class E>
+__global__ __launch_bounds__(256) void grouped_round_kernel(RoundParams p, const int32_t *offsets, int32_t experts) {
+  round_rows<E>(p, min(max(offsets[0], 0), (int)p.rows), min(max(offsets[experts], 0), (int)p.rows));
 }
 
 } // namespace zluda_amd
