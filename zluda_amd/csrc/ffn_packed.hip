@@ -37,16 +37,20 @@ uint32_t launch_rms(RmsParams p, hipStream_t s) {
     p.per_group = (int32_t)std::min<int64_t>(each * rows_each, 1 << 30);
     return launch_kernel(kernel, dim3((uint32_t)((p.rows + p.per_group - 1) / p.per_group)), dim3(threads), s, p);
   };
+  // Eight columns a thread as long as a workgroup has enough of them (sixteen and half the threads in brackets, us): 4 x 1024 2.9 (3.7), 777 x 1001 3.9 (4.8), 16384 x 1024
+  // 26.7 (28.1); 4 x 4096 3.1 (4.0), 2048 x 4096 14.4 (16.9), 16384 x 4096 110 (107); 500 x 8192 9.1 (9.5), 8192 x 8192 106 (108), packed 97.1 (97.6).  Beyond that,
+  // packed, what the many small workgroups overlap is worth more: 16384 x 8192 198 (191), plain 208 (210).
   if (p.cols <= 512) return run(rms_forward_kernel<E, 64, 4, 1>, 4, 8, 256);
-  if (p.cols <= 1024) return run(rms_forward_kernel<E, 64, 4, 2>, 4, 8, 256);
+  if (p.cols <= 1024) return run(rms_forward_kernel<E, 128, 2, 1>, 2, 8, 256);
   if (p.cols <= 2048) return run(rms_forward_kernel<E, 256, 1, 1>, 1, 8, 256);
-  if (p.cols <= 4096) return run(rms_forward_kernel<E, 256, 1, 2>, 1, 8, 256);
-  if (p.cols <= 8192) return run(rms_forward_kernel<E, 512, 1, 2>, 1, 4, 512);
+  if (p.cols <= 4096) return run(rms_forward_kernel<E, 512, 1, 1>, 1, 4, 512);
+  if (p.cols <= 8192) return p.codes && p.rows > 8192 ? run(rms_forward_kernel<E, 512, 1, 2>, 1, 4, 512) : run(rms_forward_kernel<E, 1024, 1, 1>, 1, 2, 1024);
   return run(rms_forward_kernel<E, 1024, 1, 2>, 1, 2, 1024);
 }
 
-// Rows a workgroup of the gradient kernel takes at a time, and workgroups, by the rules of the layer norm's gradient: its kernel has the same
-// shape, with one sum less
+// Rows a workgroup of the gradient kernel takes at a time, and workgroups: one round of rows while that leaves an eighth of the CUs idle, two beyond (300 x 1000 7.3 us
+// in one, 8.3 in two; 777 x 1001 8.8 and 9.2; 2000 x 512, 250 workgroups, 7.4 and 7.2: the second kernel has their sums to read), and no more workgroups than are
+// resident at once.
 int rms_grad_rows_each(uint64_t cols) { return cols <= 512 ? 8 : cols <= 1024 ? 4 : cols <= 2048 ? 2 : 1; }
 uint32_t rms_grad_groups(uint64_t rows, uint64_t cols) {
   const int each = rms_grad_rows_each(cols), least = rows <= (uint64_t)cus() * 7 / 8 * each ? each : 2 * each;
@@ -71,10 +75,7 @@ uint32_t launch_activate(const ActivateParams &p, uint32_t block_rows, hipStream
     return launch_kernel(activate_blocks_kernel<E>, grid, dim3(256), s, p);
   }
   const uint32_t strips = column_strips(p.cols);
-  auto grid = [&](int rows) { return dim3(strips, (uint32_t)std::min<int64_t>((p.rows + rows - 1) / rows, kGridY)); };
-  // four rows a thread where that still gives every CU eight workgroups
-  if (p.rows / 16 * strips >= 8 * cus()) return launch_kernel(activate_kernel<E, 4>, grid(16), dim3(256), s, p);
-  return launch_kernel(activate_kernel<E, 1>, grid(4), dim3(256), s, p);
+  return launch_kernel(activate_kernel<E>, dim3(strips, (uint32_t)std::min<int64_t>((p.rows + 3) / 4, kGridY)), dim3(256), s, p);
 }
 
 } // namespace

