@@ -32,10 +32,10 @@ def test_more_rows_than_a_grid_has(block_rows):
     back = torch.empty_like(x)
     ffn.Unpack(spec).run(codes=codes.data_ptr(), scales=scales.data_ptr(), y=back.data_ptr(), stream=stream())
     torch.cuda.synchronize()
-    rest = [slice(0, 1000), slice(rows - 256 - rows % 128, rows)]
-    for r in rest:
+    rest = [slice(0, 1024), slice(rows - 256 - rows % 128, rows)]
+    for r in rest:                                           # (whole blocks of 128 rows, whose scales are of all of them)
         value = x[r].double()
-        s = scales[:, r].t() if block_rows == 1 else scales[r.start // 128:-(-r.stop // 128)]
+        s = scales[:, r].t() if block_rows == 1 else scales[r.start // 128:-(-r.stop // 128), :1]          # (the rest of a pitch of four is nobody's)
         P.check_packed(codes[r], s, value, torch.zeros_like(value), cols, block_rows)
     # each code is off by half a step at most: 2^-4 of its value, or of the smallest normal number 2^-6 times the scale; and what it stands for, at most that much larger
     # than the value, is rounded to y's type: 2^-8 of it
