@@ -84,3 +84,12 @@ def test_workspace_of_gradients_by_expert():
     assert ffn.load().zluda_ffn_grouped_backward_workspace(C.byref(p), C.byref(n)) == K.CUBLAS_STATUS_INVALID_VALUE
     p = ffn.zluda_ffn_grouped_grad(10, 5000, 200, 300)
     assert ffn.load().zluda_ffn_grouped_backward_workspace(C.byref(p), C.byref(n)) == K.CUBLAS_STATUS_NOT_SUPPORTED
+    # pitches that are not set yet, or make no sense
+    p = ffn.zluda_ffn_grouped_grad(64, 8, 5632, 2048)
+    for name in ("dx", "dw"):
+        getattr(p, name).data = 16
+    for ld in (0, -8, -(1 << 62)):
+        for name in ("dy", "x", "w", "dx", "dw"):
+            for other in ("dy", "x", "w", "dx", "dw"):
+                getattr(p, other).ld = ld if other == name else 5632
+            assert ffn.load().zluda_ffn_grouped_backward_workspace(C.byref(p), C.byref(n)) == 0 and n.value == 0

@@ -32,4 +32,18 @@ inline float block_tiles_us(int v, uint64_t tiles, uint64_t stages, uint64_t cus
   return us * ((float)stages + t.edge);
 }
 
+// Tile configurations of the products with a scale for each 128 of K (index = plan.variant for ZLUDA_KERNEL_MFMA_BLK8): workgroup tile, waves, LDS
+// stages of 128 K bytes; uniform: only for P rows that share their scales (the accumulators of a wave leave no registers for more); exact: also for results in
+// 32 bits (the widened operands take registers)
+struct BlockVariant { int bp, bq, wp, wq, stages; bool uniform, exact; };
+constexpr BlockVariant block_variant(int v, bool uniform, bool exact) {
+  return {kBlockTiles[v].bp, kBlockTiles[v].bq, kBlockTiles[v].wp, kBlockTiles[v].wq, kBlockTiles[v].stages, uniform, exact};
+}
+constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true),
+                                           block_variant(4, false, true), block_variant(5, false, false), block_variant(6, false, false),
+                                           {16, 16, 1, 8, 0, false, true}};  // kernels/block_decode.hpp: no tile of those
+constexpr int kBlockDecode = kBlockTileCount;
+static_assert(sizeof(kBlockVariants) / sizeof(kBlockVariants[0]) == kBlockDecode + 1, "a variant each");
+constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
+
 } // namespace zluda_amd

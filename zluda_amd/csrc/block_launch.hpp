@@ -1,5 +1,6 @@
 // Launchers of the products with a scale for each 128 of K; one translation unit per pair of formats.
 #pragma once
+#include "block_cost.hpp"
 #include "kernels/block_decode.hpp"
 #include "kernels/block_gemm.hpp"
 #include "launch_util.hpp"

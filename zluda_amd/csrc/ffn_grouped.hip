@@ -112,7 +112,8 @@ GradChoice pick_grad(const zluda_ffn_grouped_grad *p) {
     auto stages = [](uint64_t k) { return (k + kGradStage - 1) / kGradStage; };
     const uint64_t n_dx = p->dx.data ? tiles(p->model) * std::max<uint64_t>(live, p->rows / side + (live + 1) / 2) : 0;
     const uint64_t n_dw = p->dw.data ? tiles(p->model) * tiles(p->features) * p->experts : 0, k_dx = stages(p->features);
-    for (uint64_t n = 1; n <= (side == 256 || !n_dx ? 1 : std::min<uint64_t>(16, k_dx)); n++) {
+    for (uint64_t n : {1, 2, 3, 4, 6, 8, 12, 16}) {
+      if (n > 1 && (side == 256 || !n_dx || n_dx >= slots || n > k_dx)) break;
       const double us = grad_together_stages(slots, n_dx, k_dx, n_dw, stages(p->rows / p->experts), n, pace) * (side == 256 ? 1.65 : 1.0);
       if (best.side && us >= best_us) continue;
       best = {side, 1, (uint32_t)((k_dx + n - 1) / n), 0};
@@ -126,10 +127,10 @@ GradChoice pick_grad(const zluda_ffn_grouped_grad *p) {
 
 // the same for the gradients, through windows of 2 GiB on an expert's matrices and rows; whole pieces of eight along every row
 bool tile_shapes(const zluda_ffn_grouped_grad *p) {
-  int64_t ld = p->dy.ld, most = p->dy.ld;
-  if (p->dx.data) { ld |= p->w.ld | p->dx.ld; most = std::max({most, p->w.ld, p->dx.ld}); }
-  if (p->dw.data) { ld |= p->x.ld | p->dw.ld; most = std::max({most, p->x.ld, p->dw.ld}); }
-  if ((ld & 7) || (p->model & 7) || (p->features & 7) || most >= kNarrowPitch || most < 1) return false;
+  int64_t ld = p->dy.ld, most = p->dy.ld, least = p->dy.ld;  // (a workspace is asked for before pitches are checked)
+  if (p->dx.data) { ld |= p->w.ld | p->dx.ld; most = std::max({most, p->w.ld, p->dx.ld}); least = std::min({least, p->w.ld, p->dx.ld}); }
+  if (p->dw.data) { ld |= p->x.ld | p->dw.ld; most = std::max({most, p->x.ld, p->dw.ld}); least = std::min({least, p->x.ld, p->dw.ld}); }
+  if ((ld & 7) || (p->model & 7) || (p->features & 7) || most >= kNarrowPitch || least < 1) return false;
   return in_window(p->rows, p->dy.ld) && (!p->dx.data || in_window(p->features, p->w.ld)) && (!p->dw.data || in_window(p->rows, p->x.ld));
 }
 bool tile_operands(const zluda_ffn_grouped_grad *p) {

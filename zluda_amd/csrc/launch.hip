@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "block_cost.hpp"
 #include "decode_launch.hpp"
 #include "launch_util.hpp"
 #include "kernels/aux_epilogue.hpp"

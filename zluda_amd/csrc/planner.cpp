@@ -3,6 +3,7 @@
 // The accepted surface follows the reference's (zluda_blaslt/src/impl.rs:257-305 for the
 // attributes, zluda_common/src/lib.rs:575-630 for the type maps) extended by what the quantized
 // path needs: scale pointers/modes, pointer modes, FP4/UE8M0 types.
+#include "block_cost.hpp"
 #include "planner.hpp"
 
 #include "kernels/store_window.hpp"

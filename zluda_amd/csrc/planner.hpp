@@ -2,7 +2,6 @@
 #pragma once
 #include "../../include/cublaslt_abi.h"
 #include "../../include/zluda_gemm_launch.h"
-#include "block_cost.hpp"
 #include "gemm_args.hpp"
 
 namespace zluda_amd {
@@ -52,19 +51,6 @@ constexpr int kTr64Stages[] = {6, 3, 2};  // and of variant 2: up to one workgro
 constexpr int tr_ring_stages(int variant, uint64_t groups, uint64_t cus) {
   return variant == 1 ? (groups <= cus ? kTrDeepStages : 2) : variant == 2 ? kTr64Stages[groups <= cus ? 0 : groups <= 3 * cus ? 1 : 2] : 2;
 }
-// tile configurations of the products with a scale for each 128 of K (index = plan.variant for ZLUDA_KERNEL_MFMA_BLK8): workgroup tile, waves, LDS
-// stages of 128 K bytes; uniform: only for P rows that share their scales (the accumulators of a wave leave no registers for more); exact: also for results in
-// 32 bits (the widened operands take registers)
-struct BlockVariant { int bp, bq, wp, wq, stages; bool uniform, exact; };
-constexpr BlockVariant block_variant(int v, bool uniform, bool exact) {
-  return {kBlockTiles[v].bp, kBlockTiles[v].bq, kBlockTiles[v].wp, kBlockTiles[v].wq, kBlockTiles[v].stages, uniform, exact};
-}
-constexpr BlockVariant kBlockVariants[] = {block_variant(0, true, false), block_variant(1, false, false), block_variant(2, false, true), block_variant(3, false, true),
-                                           block_variant(4, false, true), block_variant(5, false, false), block_variant(6, false, false),
-                                           {16, 16, 1, 8, 0, false, true}};  // kernels/block_decode.hpp: no tile of those
-constexpr int kBlockDecode = kBlockTileCount;
-static_assert(sizeof(kBlockVariants) / sizeof(kBlockVariants[0]) == kBlockDecode + 1, "a variant each");
-constexpr int kNumBlockVariants = sizeof(kBlockVariants) / sizeof(kBlockVariants[0]);
 constexpr int kNumTrVariants = sizeof(kTrVariants) / sizeof(kTrVariants[0]);
 
 // decode configurations (index = plan.variant for ZLUDA_KERNEL_DECODE_W8A8).
