@@ -45,7 +45,7 @@ uint32_t launch_rms(RmsParams p, hipStream_t s) {
   if (p.cols <= 2048) return run(rms_forward_kernel<E, 256, 1, 1>, 1, 8, 256);
   if (p.cols <= 4096) return run(rms_forward_kernel<E, 512, 1, 1>, 1, 4, 512);
   if (p.cols <= 8192) return p.codes && p.rows > 8192 ? run(rms_forward_kernel<E, 512, 1, 2>, 1, 4, 512) : run(rms_forward_kernel<E, 1024, 1, 1>, 1, 2, 1024);
-  return run(rms_forward_kernel<E, 1024, 1, 2>, 1, 2, 1024);
+  return run(rms_forward_kernel<E, 1024, 1, 2>, 1, 1, 1024);
 }
 
 // Rows a workgroup of the gradient kernel takes at a time, and workgroups: one round of rows while that leaves an eighth of the CUs idle, two beyond (300 x 1000 7.3 us

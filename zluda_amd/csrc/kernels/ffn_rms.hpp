@@ -26,8 +26,10 @@ struct RmsParams {
   uint32_t weight_type;
 };
 
+// (Eight waves a SIMD, so that the workgroups a launch counts on are there at once: f32 has registers for seven otherwise, 2000 x 4096 29.0 us, 27.7.  Groups of fewer lanes
+// would spill for it, a workgroup more or less of theirs is not seen.)
 template <class E, int T, int R, int NV>
-__global__ __launch_bounds__(T *R) void rms_forward_kernel(RmsParams p) {
+__global__ __launch_bounds__(T *R, NV == 1 && T >= 256 ? 8 : 4) void rms_forward_kernel(RmsParams p) {
   using raw = typename E::raw;
   __shared__ float words[2][R][T / 64][2];
   const int lane = threadIdx.x % T, group = threadIdx.x / T;
