@@ -47,6 +47,33 @@ def test_shares_of_a_long_k(typ, counts, spare, f, d):
         O.check(dw.view[q], P.product(dy.view[r].double().t(), x.view[r].double().t()), "dw, expert %d" % i)
 
 
+@pytest.mark.parametrize("f,d", [(64, 72), (40, 33)])
+def test_most_experts(f, d):
+    """as many experts as there may be, few of which have rows"""
+    counts = [0] * 4096
+    for e, n in ((0, 3), (63, 1), (64, 2), (1000, 70), (2047, 1), (2048, 130), (4094, 5), (4095, 1)):
+        counts[e] = n
+    o, dev = offsets_of(counts)
+    rows, live = o[-1] + 2, [e for e in range(4096) if counts[e]]
+    x, dy, w = randn(1, rows, d).to(BF[0]), randn(2, rows, f).to(BF[0]), randn(3, 4096 * f, d, std=d ** -0.5).to(BF[0])
+    y, dx, dw = torch.full_like(dy, 7), torch.full_like(x, 7), torch.full_like(w, 7)
+    spec = dict(type=BF[1], rows=rows, experts=4096, features=f, model=d)
+    fwd, bwd = ffn.GroupedForward(spec), ffn.GroupedBackward(spec)
+    ws = torch.empty(max(16, bwd.workspace), dtype=torch.uint8, device=DEV)
+    fwd.run(offsets=dev.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), y=y.data_ptr(), stream=stream())
+    bwd.run(offsets=dev.data_ptr(), dy=dy.data_ptr(), x=x.data_ptr(), w=w.data_ptr(), dx=dx.data_ptr(), dw=dw.data_ptr(), workspace=ws.data_ptr(), workspace_size=ws.numel(),
+            stream=stream())
+    torch.cuda.synchronize()
+    for e in live:
+        r, q = slice(o[e], o[e + 1]), slice(e * f, (e + 1) * f)
+        O.check(y[r], P.product(x[r].double(), w[q].double()), "y")
+        O.check(dx[r], P.product(dy[r].double(), w[q].double().t()), "dx")
+        O.check(dw[q], P.product(dy[r].double().t(), x[r].double().t()), "dw")
+    assert (y[-2:] == 7).all() and (dx[-2:] == 7).all()
+    others = dw.view(4096, f, d)[[e for e in range(4096) if not counts[e]]]
+    assert not others.any()
+
+
 BAD = [float("nan"), float("inf"), -float("inf")]
 
 
