@@ -209,3 +209,15 @@ def test_codes_beyond_4_gib(gpu_api):
     torch.cuda.synchronize()
     O.check(y, P.scaled_product(x.double(), values(w), P.spread(xs.t().double(), n, k), sw))
     call.close()
+
+
+def test_gradients_on_two_streams_at_once():
+    """two backward passes with shares of K, each with its own workspace, neither on the current stream"""
+    passes, streams = [grouped_pass([30, 0, 40], 2816, 520, 3), grouped_pass([64], 4096, 1024, 4)], [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for (run, _, _, _), s in zip(passes, streams):
+            run(s.cuda_stream)
+    torch.cuda.synchronize()
+    for (_, check, _, _), counts in zip(passes, ([30, 0, 40], [64])):
+        check(counts, str(counts))
