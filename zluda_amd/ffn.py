@@ -17,7 +17,8 @@ A call object is configured once with a plain dict (types, sizes, pitches) and r
   Activate       type, rows, cols; activation (SILU, GELU, RELU, COPY; default SILU), block_rows (1 or 128; default 1)
   Unpack         type, rows, cols; block_rows
   GroupedForward   type (of x, w and y; packed: of y), rows, experts, model, features; packed (bool)
-  GroupedBackward  type, rows, experts, model, features; outputs, wanted by default: dx, dw (bool)
+  GroupedBackward  type, rows, experts, model, features; outputs, wanted by default: dx, dw (bool).  run() may leave one out; dx alone can take more scratch
+                   than both of them do (its sums are shared out further): `workspace_dx` bytes
 
 A call object writes the addresses into its own structure and hands that to the library: one thread at a time may run it (several threads: an object each).
 `workspace` is the number of bytes of device scratch that run() wants.  Pitches default to tight rows, those of checkpoints to what
@@ -409,10 +410,17 @@ class GroupedBackward(_Call):
             self.matrix(name, cols, t)
         for name in ("dx", "dw"):
             getattr(p, name).data = 16 if s.get(name, True) else None
+        wanted = p.dx.data, p.dw.data
+        p.dx.data, p.dw.data = 16, None
+        self.query(self.lib.zluda_ffn_grouped_backward_workspace)
+        self.workspace_dx = self.workspace
+        p.dx.data, p.dw.data = wanted
         self.query(self.lib.zluda_ffn_grouped_backward_workspace)
         self._call, self._ref, self._m = self.lib.zluda_ffn_grouped_backward, C.byref(p), _members(p, "dy x w dx dw")
 
     def run(self, offsets, dy, x=None, w=None, dx=None, dw=None, workspace=None, workspace_size=0, stream=None):
+        if dx and not dw and workspace_size < self.workspace_dx:
+            raise cublaslt.CublasLtError(abi.CUBLAS_STATUS_ALLOC_FAILED, "zluda_ffn_grouped_backward of dx alone, which takes a workspace of %d bytes," % self.workspace_dx)
         my, mx, mw, mdx, mdw = self._m
         self.p.offsets, my.data, mx.data, mw.data, mdx.data, mdw.data = offsets, dy, x, w, dx, dw
         status = self._call(self._ref, workspace, workspace_size, stream)
