@@ -1,4 +1,4 @@
-"""zluda_amd.expert_block in 8 bits, operator by operator: each against the definition in 64 bits of what the one in front of it left."""
+"""zluda_amd.expert_block in 8 bits, operator by operator: each against the definition in 64 bits of what the one in front of it left; and which calls may follow it."""
 import pytest
 import torch
 
@@ -61,3 +61,20 @@ def test_operator_by_operator(gpu_api, dtype, tokens, model, features, experts, 
     back = back.reshape(tokens, top, model)
     value, mag = block.s.double() + back.sum(1), block.s.double().abs() + back.abs().sum(1)
     O.check(out, (value, (top + 2) * 2 * O.E32 * mag), "out")
+
+
+def test_no_gradients_of_an_8_bit_pass(gpu_api):
+    """what the 8-bit pass leaves is not what backward() reads: it says so, until the next forward()"""
+    block, x, residual, chosen, share, dout = expert_block.example(40, 128, 96, 4, 2)
+    with pytest.raises(RuntimeError):
+        block.backward(dout)
+    block.pack()
+    block.forward(x, residual, chosen, share)
+    first = [t.clone() for t in block.backward(dout)] + [g.clone() for g in block.grads.values()]
+    block.forward8(x, residual, chosen, share)
+    with pytest.raises(RuntimeError):
+        block.backward(dout)
+    block.forward(x, residual, chosen, share)
+    again = list(block.backward(dout)) + list(block.grads.values())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(first, again))

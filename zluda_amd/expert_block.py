@@ -49,6 +49,7 @@ class ExpertBlock:
         calls = (self.norm_backward, self.activate_backward, self.up, self.up_backward, self.down, self.down_backward, self.up8, self.down8)
         self.workspace = torch.empty(max(16, *(c.workspace for c in calls)), dtype=torch.uint8, device=device)
         self.codes_n, self.codes_h = ffn.packed_buffers(tokens, model, device), ffn.packed_buffers(rows, features, device)
+        self.share = None
 
     def _scratch(self):
         return dict(workspace=self.workspace.data_ptr(), workspace_size=self.workspace.numel(), stream=_stream())
@@ -80,7 +81,9 @@ class ExpertBlock:
         return self._bring_back(self.s, self.y, share)
 
     def backward(self, dout):
-        """gradients of sum(dout * out): the parameters' in `grads`; x's (and residual's) and share's are returned"""
+        """gradients of sum(dout * out) of the forward() before it: the parameters' in `grads`; x's (and residual's) and share's are returned"""
+        if self.share is None:
+            raise RuntimeError("backward() reads what forward() left: there was none, or forward8() has written over it")
         p, g, offsets = self.params, self.grads, self.offsets.data_ptr()
         rows = dout[self.token].float()
         dshare = torch.empty(self.order.numel(), device=self.device)
@@ -107,7 +110,8 @@ class ExpertBlock:
         self.w8, self.d8 = packed(self.params["w"]), packed(self.params["down"])
 
     def forward8(self, x, residual, chosen, share):
-        """forward() with both products in 8 bits; pack() first"""
+        """forward() with both products in 8 bits; pack() first, and again when the parameters have changed"""
+        self.share = None  # (z and y are what backward() would read)
         self._sort(chosen)
         offsets, (nc, ns), (hc, hs) = self.offsets.data_ptr(), self.codes_n, self.codes_h
         self.norm_forward.run(x=x.data_ptr(), residual=residual.data_ptr(), weight=self.params["norm_weight"].data_ptr(), sum=self.s.data_ptr(), codes=nc.data_ptr(),
