@@ -27,7 +27,7 @@ class ExpertBlock:
         gen.manual_seed(seed)
         rand = lambda *s, std: (torch.randn(s, device=device, generator=gen) * std).to(dtype)  # noqa: E731
         empty = lambda *s, t=dtype: torch.empty(s, dtype=t, device=device)  # noqa: E731
-        self.top, self.experts, self.features, self.device = top, experts, features, device
+        self.top, self.experts, self.features, self.device, self.shape = top, experts, features, device, (tokens, model)
         rows, typ = tokens * top, _TYPES[dtype]
         self.params = {"norm_weight": torch.ones(model, device=device), "w": rand(experts, 2 * features, model, std=model ** -0.5),
                        "down": rand(experts, model, features, std=features ** -0.5)}
@@ -51,6 +51,15 @@ class ExpertBlock:
         self.codes_n, self.codes_h = ffn.packed_buffers(tokens, model, device), ffn.packed_buffers(rows, features, device)
         self.share = None
 
+    def _check(self, chosen=None, share=None, **matrices):
+        """the operators take addresses: what they are not told must be so"""
+        for name, t in matrices.items():
+            if tuple(t.shape) != self.shape or t.dtype != self.s.dtype or t.device != self.s.device or not t.is_contiguous():
+                raise ValueError("%s: a contiguous tensor of %d x %d, %s, on %s" % (name, *self.shape, self.s.dtype, self.s.device))
+        for name, t in (("chosen", chosen), ("share", share)):
+            if t is not None and tuple(t.shape) != (self.shape[0], self.top):
+                raise ValueError("%s: %d x %d" % (name, self.shape[0], self.top))
+
     def _scratch(self):
         return dict(workspace=self.workspace.data_ptr(), workspace_size=self.workspace.numel(), stream=_stream())
 
@@ -69,6 +78,7 @@ class ExpertBlock:
         return (base.float() + back.reshape(base.shape[0], self.top, -1).sum(1)).to(base.dtype)
 
     def forward(self, x, residual, chosen, share):
+        self._check(chosen, share, x=x, residual=residual)
         self._sort(chosen)
         p, offsets = self.params, self.offsets.data_ptr()
         self.norm_forward.run(x=x.data_ptr(), residual=residual.data_ptr(), weight=p["norm_weight"].data_ptr(), sum=self.s.data_ptr(), y=self.n.data_ptr(),
@@ -84,6 +94,7 @@ class ExpertBlock:
         """gradients of sum(dout * out) of the forward() before it: the parameters' in `grads`; x's (and residual's) and share's are returned"""
         if self.share is None:
             raise RuntimeError("backward() reads what forward() left: there was none, or forward8() has written over it")
+        self._check(dout=dout)
         p, g, offsets = self.params, self.grads, self.offsets.data_ptr()
         rows = dout[self.token].float()
         dshare = torch.empty(self.order.numel(), device=self.device)
@@ -111,6 +122,7 @@ class ExpertBlock:
 
     def forward8(self, x, residual, chosen, share):
         """forward() with both products in 8 bits; pack() first, and again when the parameters have changed"""
+        self._check(chosen, share, x=x, residual=residual)
         self.share = None  # (z and y are what backward() would read)
         self._sort(chosen)
         offsets, (nc, ns), (hc, hs) = self.offsets.data_ptr(), self.codes_n, self.codes_h
