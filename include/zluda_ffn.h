@@ -195,8 +195,9 @@ uint32_t zluda_ffn_grouped_forward_workspace(const zluda_ffn_grouped *p, size_t 
 
 /* The gradients, all matrices of one 16-bit type:
  *   dx[r] = W_e^T dy[r] (rows x model)      dw: dW_e = sum over the rows of e of dy[r]^T x[r] (experts * features x model), zeros for an expert without rows
- * dx or dw may be absent; w is needed for dx, x for dw.  Neither may be one of the operands.  Few rows share out dx's sums, which takes a workspace: it is asked
- * for with the sizes, the pitches and which of dx and dw there will be.  Sums are taken in a fixed order: the same bits in every call. */
+ * dx or dw may be absent; w is needed for dx, x for dw.  Neither may be one of the operands.  Few rows share out dx's sums, which takes a workspace, 16-byte
+ * aligned: it is asked for with the sizes, the pitches and which of dx and dw there will be (dx alone can take more than both), and does not depend on addresses.
+ * Sums are taken in a fixed order: the same bits in every call. */
 typedef struct zluda_ffn_grouped_grad {
   uint64_t rows, experts, features, model;
   const int32_t *offsets;

@@ -175,7 +175,7 @@ extern "C" uint32_t zluda_ffn_grouped_backward(const zluda_ffn_grouped_grad *p, 
   const GradChoice pick = pick_grad(p);
   const uint64_t need = tile_shapes(p) ? pick.part : 0;
   if (need > workspace_size || (need && !workspace)) return CUBLAS_STATUS_ALLOC_FAILED;
-  if ((uintptr_t)workspace & 15) return CUBLAS_STATUS_INVALID_VALUE;
+  if (need && ((uintptr_t)workspace & 15)) return CUBLAS_STATUS_INVALID_VALUE;
   if (!zluda_gemm_device_cu_count()) return CUBLAS_STATUS_NOT_INITIALIZED;
   const hipStream_t s = (hipStream_t)stream;
   if (tile_operands(p)) {

@@ -126,7 +126,7 @@ extern "C" uint32_t zluda_ffn_rms_backward(const zluda_ffn_rms_grad *p, void *wo
   size_t need = 0;
   FFN_CHECK(zluda_ffn_rms_backward_workspace(p, &need));
   if (need > workspace_size || (need && !workspace)) return CUBLAS_STATUS_ALLOC_FAILED;
-  if ((uintptr_t)workspace & 15) return CUBLAS_STATUS_INVALID_VALUE;
+  if (need && ((uintptr_t)workspace & 15)) return CUBLAS_STATUS_INVALID_VALUE;
   if (!zluda_gemm_device_cu_count()) return CUBLAS_STATUS_NOT_INITIALIZED;
   const hipStream_t s = (hipStream_t)stream;
   if (!p->rows) {  // a sum of no terms
