@@ -3,6 +3,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "../../include/zluda_ffn.h"
 #include "../../include/zluda_gemm_launch.h"
 #include "ffn_launch.hpp"
 #include "launch_util.hpp"
@@ -25,5 +26,11 @@ inline int cus() {
   } while (0)
 
 inline uint32_t check_vector(const void *v, uint32_t type) { return ((uintptr_t)v & (elem_size(type) - 1)) ? CUBLAS_STATUS_INVALID_VALUE : CUBLAS_STATUS_SUCCESS; }
+// a matrix of plain elements that has to be there
+inline uint32_t check_plain(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, uint32_t type) {
+  if (!m.data && rows) return CUBLAS_STATUS_INVALID_VALUE;
+  if (m.type != type) return CUBLAS_STATUS_NOT_SUPPORTED;
+  return m.ld < (int64_t)cols || ((uintptr_t)m.data & (elem_size(type) - 1)) ? CUBLAS_STATUS_INVALID_VALUE : CUBLAS_STATUS_SUCCESS;
+}
 
 } // namespace zluda_amd

@@ -1,9 +1,8 @@
 // The entry points of include/zluda_ffn.h for products grouped by expert: argument checks, kernel choice and launches.
-#include <cmath>
-
 #include "../../include/zluda_ffn.h"
 
 #include "ffn_checks.hpp"
+#include "ffn_grouped_choice.hpp"
 #include "ffn_grouped_launch.hpp"
 #include "planner.hpp"
 
@@ -14,11 +13,6 @@ namespace {
 uint32_t check_sizes(uint64_t rows, uint64_t experts, uint64_t features, uint64_t model, const int32_t *offsets) {
   if (!experts || !features || !model || ((uintptr_t)offsets & 3) || !offsets) return CUBLAS_STATUS_INVALID_VALUE;
   return rows > kMaxSide || experts > ZLUDA_FFN_MAX_EXPERTS || features > kMaxFeatures || model > kMaxFeatures ? CUBLAS_STATUS_NOT_SUPPORTED : CUBLAS_STATUS_SUCCESS;
-}
-uint32_t check_plain(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, uint32_t type) {
-  if (!m.data && rows) return CUBLAS_STATUS_INVALID_VALUE;
-  if (m.type != type) return CUBLAS_STATUS_NOT_SUPPORTED;
-  return m.ld < (int64_t)cols || ((uintptr_t)m.data & (elem_size(type) - 1)) ? CUBLAS_STATUS_INVALID_VALUE : CUBLAS_STATUS_SUCCESS;
 }
 
 uint32_t check_forward(const zluda_ffn_grouped *p) {
@@ -68,30 +62,6 @@ bool tile_operands(const zluda_ffn_grouped *p) {
   return aligned && near;
 }
 
-// The tile whose last workgroup is done first, if the rows are shared out about evenly, which only the device knows: a tile for each expert, and beyond that half
-// of one that is not full for each, give or take `spread`: half of the estimate is the time with that much more, where a tile that fills the chip exactly goes into a
-// second round (1001 rows of eight experts, 1024 x 2816, six draws of their counts: 14.4 to 15.2 us; without it 13.6 to 22.1).  Measured, us, in the order of kBlockTiles: 2048 of model, 5632 features, eight experts, bf16, 16 rows 53, 42, 37, 35, 39 and 46; 256 58,
-// 45, 39, 41, 42 and 48; 1024 65, 68, 66, 78, 59, 59; 2048 94, 83, 108, 129, 91, 84; 4096 118, 140, 174, 220, 148, 142; 1024 of model, 2816 features, 64 experts, 4096 rows
-// 103, 91, 97, 105, 87, 93.
-int pick_tile(const zluda_ffn_grouped *p) {
-  const bool eight = p->x.type == CUDA_R_8F_E4M3, exact = eight && p->y.type == CUDA_R_32F;
-  const uint64_t live = std::min(p->rows, p->experts), stages = (p->model * (eight ? 1 : 2) + 127) / 128;
-  const uint64_t spread = live > 1 ? (uint64_t)std::ceil(0.29 * std::sqrt((double)live)) : 0;  // (a part of a tile each, even chances: 1 / sqrt(12) of a tile)
-  int best = -1;
-  float best_us = 0.0f;
-  for (int v = 0; v < kBlockTileCount; v++) {
-    if (exact && !kBlockVariants[v].exact) continue;
-    const uint64_t q = std::max<uint64_t>(live, p->rows / kBlockTiles[v].bq + (live + 1) / 2), across = (p->features + kBlockTiles[v].bp - 1) / kBlockTiles[v].bp;
-    float us = block_tiles_us(v, q * across, stages, (uint64_t)cus(), eight);
-    if (q > live) us = 0.5f * (us + block_tiles_us(v, (q + spread) * across, stages, (uint64_t)cus(), eight));
-    if (best < 0 || us < best_us) {
-      best = v;
-      best_us = us;
-    }
-  }
-  return best;
-}
-
 // Tiles of 128 x 128, two workgroups a CU, with dx's K in as many shares as grad_together_stages() has done first, or of 256 x 256; a stage takes 1.0 and 1.65 us.
 // Measured, us, 1 share, 2, 4, 8, tiles of 256: 64 rows of eight experts, 2048 of model, 5632 features 106, 86, 98, 98, 149; 1024 123, 117, 127, 146, 160; 300,
 // eight, 1024 x 2816 50, 37, 31, 31, 70; 692, two, 2688 x 4744 83, 68, 71, 84, 115; 64, one, 4096 x 4096 43, 29, 21, 23, 60; 600, 16, 2048 x 1408 46, 59, 65, 69, 49;
@@ -103,6 +73,7 @@ struct GradChoice {
   uint64_t part;                    // bytes of their sums
 };
 GradChoice pick_grad(const zluda_ffn_grouped_grad *p) {
+  // (pace: a stage of a share waits for W, the longer where W and dW are more than the memory-side cache; as for the gated layer, grad_together())
   const uint64_t live = std::max<uint64_t>(1, std::min(p->rows, p->experts)), pace = 4 * p->experts * p->features * p->model > 256ull << 20 ? 2 : 1;
   GradChoice best{0, 1, 0, 0};
   double best_us = 0.0;
@@ -155,7 +126,7 @@ extern "C" uint32_t zluda_ffn_grouped_forward(const zluda_ffn_grouped *p, void *
   const GroupedParams g{p->offsets, p->x.data, p->w.data, p->y.data, (const float *)p->x.scales, (const float *)p->w.scales, p->x.ld, p->w.ld, p->y.ld,
                         p->x.ld_scales, p->w.ld_scales, (int32_t)p->rows, (int32_t)p->experts, (int32_t)p->features, (int32_t)p->model, p->x.type, p->y.type};
   if (tile_operands(p)) {
-    const int tile = pick_tile(p);
+    const int tile = grouped_tile(p, (uint64_t)cus());
     if (((p->features + kBlockTiles[tile].bp - 1) / kBlockTiles[tile].bp) * most_row_tiles(p->rows, p->experts, kBlockTiles[tile].bq) < (1ull << 31))
       return (p->x.type == CUDA_R_16BF ? launch_grouped_bf16 : p->x.type == CUDA_R_16F ? launch_grouped_f16 : launch_grouped_f8)(g, tile, (hipStream_t)stream);
   }

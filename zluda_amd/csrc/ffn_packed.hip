@@ -11,11 +11,6 @@ namespace {
 
 bool plain_type(uint32_t type) { return is_h16(type) || type == CUDA_R_32F; }
 
-uint32_t check_plain(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, uint32_t type) {
-  if (!m.data && rows) return CUBLAS_STATUS_INVALID_VALUE;
-  if (m.type != type) return CUBLAS_STATUS_NOT_SUPPORTED;
-  return m.ld < (int64_t)cols || ((uintptr_t)m.data & (elem_size(type) - 1)) ? CUBLAS_STATUS_INVALID_VALUE : CUBLAS_STATUS_SUCCESS;
-}
 uint32_t check_packed(const zluda_ffn_matrix &m, uint64_t rows, uint64_t cols, uint32_t block_rows) {
   if ((!m.data || !m.scales) && rows) return CUBLAS_STATUS_INVALID_VALUE;
   if (m.type != CUDA_R_8F_E4M3) return CUBLAS_STATUS_NOT_SUPPORTED;
