@@ -48,7 +48,7 @@ extern "C" {
  * element (r, c) is at scales[c / 128 * ld_scales + r], ld_scales >= rows (blocks of 128 rows: at scales[r / 128 * ld_scales + c / 128],
  * ld_scales >= ceil(columns / 128)): with ld_scales the rows what CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F takes, with
  * ceil(columns / 128) rounded up to four what BLK128x128_32F takes.  data may lie anywhere (rows on 16 bytes are the fast case); nothing behind a
- * row's last column is written. */
+ * row's last column is written.  Products multiply by the product of two scales, in 32 bits, which has to be finite. */
 typedef struct zluda_ffn_matrix {
   void *data;
   void *scales;      /* checkpoints and what is packed */
@@ -134,7 +134,7 @@ uint32_t zluda_ffn_checkpoint_load(uint64_t rows, uint64_t cols, const zluda_ffn
  * The norm takes the rounded h, which is what the backward pass reads.  x, residual, sum (receives h), y: rows x cols of one type (16F, 16BF, 32F), cols up
  * to 16384; packed receives y packed, from its 32-bit values; sum, y and packed are absent or wanted (data == NULL), one of them at least wanted;
  * weight: cols elements of weight_type (x's or 32F), NULL: 1; rstd: rows floats or NULL.  sum or y may be x or residual itself, with its
- * pitch, but sum is not y. */
+ * pitch, but sum is not y.  Squares and their sum are held in 32 bits: a row whose sum of squares passes 2^128 has rstd 0. */
 typedef struct zluda_ffn_rms {
   uint64_t rows, cols;
   float eps;
@@ -181,8 +181,12 @@ uint32_t zluda_ffn_unpack(uint64_t rows, uint64_t cols, uint32_t block_rows, con
  * memory that do not decrease, from 0 to rows; an expert may have none, and rows that no expert has stay as they are in y and dx.
  *   y[r] = W_e x[r]      x: rows x model, w: experts * features x model (expert e: rows e * features and on), y: rows x features
  * x, w and y of one 16-bit type; or x packed, w packed in blocks of 128 x 128 that start anew at each expert (scales of expert e from block row
- * e * ceil(features / 128) on), and y 16F, 16BF or 32F.  Sums in 32 bits.  Numbers in offsets that break the rule give wrong results, but nothing outside
- * the matrices is touched. */
+ * e * ceil(features / 128) on), and y 16F, 16BF or 32F.  y is none of the operands.  Numbers in offsets that break the rule give wrong results, but nothing outside
+ * the matrices is touched.
+ * Sums in 32 bits.  Packed operands with a 16-bit y are multiplied by the 8-bit instruction, which drops of each eight neighbouring products what lies 2^13 below the
+ * largest: 1.4e-5 of a result (2-norm), below its rounding.  For y of 32F they are multiplied by the 16-bit one, which does not, at half the rate.
+ * model a multiple of eight (packed: of 16), x and w with their rows on 16 bytes: tiles on the matrix units.  Anything else, and pitches of 2^22 and more: a kernel on
+ * the vector units, 13 to 29 times as long (1001 rows of eight, 1024 x 2816: 241 us for 15.5). */
 #define ZLUDA_FFN_MAX_EXPERTS 4096u
 typedef struct zluda_ffn_grouped {
   uint64_t rows, experts, features, model;
@@ -197,7 +201,9 @@ uint32_t zluda_ffn_grouped_forward_workspace(const zluda_ffn_grouped *p, size_t 
  *   dx[r] = W_e^T dy[r] (rows x model)      dw: dW_e = sum over the rows of e of dy[r]^T x[r] (experts * features x model), zeros for an expert without rows
  * dx or dw may be absent; w is needed for dx, x for dw.  Neither may be one of the operands.  Few rows share out dx's sums, which takes a workspace, 16-byte
  * aligned: it is asked for with the sizes, the pitches and which of dx and dw there will be (dx alone can take more than both), and does not depend on addresses.
- * Sums are taken in a fixed order: the same bits in every call. */
+ * Sums are taken in a fixed order: the same bits in every call.  model, features and all pitches multiples of eight, addresses of 16 bytes, and rows x the pitch of
+ * dy and of x below 2 GiB (features x the pitch of w too): tiles on the matrix units.  Anything else: the vector units (eight experts, 1024 x 28672: 37000 rows 3.4 ms,
+ * 40000, beyond 2 GiB, 135 ms). */
 typedef struct zluda_ffn_grouped_grad {
   uint64_t rows, experts, features, model;
   const int32_t *offsets;
