@@ -75,7 +75,7 @@ class ExpertBlock:
         rows = rows.float() if share is None else rows.float() * share.reshape(-1, 1)[self.order]
         back = torch.empty_like(rows)
         back[self.order] = rows
-        return (base.float() + back.reshape(base.shape[0], self.top, -1).sum(1)).to(base.dtype)
+        return (base.float() + back.reshape(base.shape[0], self.top, base.shape[1]).sum(1)).to(base.dtype)
 
     def forward(self, x, residual, chosen, share):
         self._check(chosen, share, x=x, residual=residual)
