@@ -149,7 +149,8 @@ typedef uint32_t cublasLtMatmulDescAttributes_t;
 /* 8-bit float operands, both of them: one float for each 128 of K (L = ceil(K / 128) of them), of a row of op(A) or a column of op(B), ...
  * scale of row i at [k / 128 * rows + i], the scales of a batch behind those of the one before */
 #define CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F 4
-/* ... or of 128 such rows: at [i / 128 * L4 + k / 128], L4 the multiple of four from L on.  The product of an A and a B scale is taken in 32 bits and has to be finite. */
+/* ... or of 128 such rows: at [i / 128 * L4 + k / 128], L4 the multiple of four from L on.  The product of an A and a B scale is
+ * held in 32 bits: finite, and a normal number wherever the result is to keep its precision. */
 #define CUBLASLT_MATMUL_MATRIX_SCALE_BLK128x128_32F 5
 
 /* ---- cublasLtEpilogue_t : cuda_types/src/cublaslt.rs:4547-4660 --------------------------- */

@@ -48,7 +48,8 @@ extern "C" {
  * element (r, c) is at scales[c / 128 * ld_scales + r], ld_scales >= rows (blocks of 128 rows: at scales[r / 128 * ld_scales + c / 128],
  * ld_scales >= ceil(columns / 128)): with ld_scales the rows what CUBLASLT_MATMUL_MATRIX_SCALE_VEC128_32F takes, with
  * ceil(columns / 128) rounded up to four what BLK128x128_32F takes.  data may lie anywhere (rows on 16 bytes are the fast case); nothing behind a
- * row's last column is written.  Products multiply by the product of two scales, in 32 bits, which has to be finite. */
+ * row's last column is written.  Products multiply by the product of two scales, held in 32 bits: finite, and a
+ * normal number wherever the result is to keep its precision (a block of zeros has the scale 2^-126: its products are zeros all the same). */
 typedef struct zluda_ffn_matrix {
   void *data;
   void *scales;      /* checkpoints and what is packed */
